@@ -341,6 +341,126 @@ int qmv_device_rms_norm_f32(const float *d_input, const float *d_weight,
 int qmv_device_greedy_argmax_f32(const float *d_logits, int vocab_size,
                                  int *d_result, void *stream);
 
+/* ---- Attention between the projections ----------------------------------- */
+
+/*
+ * The tokens of a step, packed sequence after sequence, as device arrays.
+ * Sequence s brings the tokens starts[s] .. starts[s + 1] - 1 of the call's
+ * `tokens` and has lengths[s] tokens with them, so its new token i stands at
+ * position lengths[s] - (starts[s + 1] - starts[s]) + i. Page p of a
+ * sequence's cache is the cache's page pages[s * table_stride + p]. The arrays
+ * are read on the device: a step that is captured in a graph may be replayed
+ * with other contents. starts has to rise (or stay) from 0 or more to `tokens`
+ * or less; what it says beyond those is cut to them. Tokens that no sequence
+ * has are left out: their rows of the outputs stay as they were.
+ */
+typedef struct QmvSequences {
+    const int *starts;  /* [count + 1] */
+    const int *lengths; /* [count]; null: the new tokens are all there are */
+    const int *pages;   /* [count][table_stride]; null where there is no cache */
+    int count;          /* 1 .. 65535 */
+    int table_stride;   /* pages a sequence may have */
+} QmvSequences;
+
+/*
+ * Keys and values of one layer, in pages of page_size tokens. The D values of
+ * token t, head h of page p begin at element p * page_stride + h * head_stride
+ * + t * token_stride of keys and of values, so pages may hold [head][token][D]
+ * or [token][head][D], and keys and values may share an allocation. type is
+ * a GGML code: QMV_TYPE_F32, QMV_TYPE_F16 or QMV_TYPE_BF16. The strides are
+ * multiples of 8 elements and at least D; keys and values are aligned to 16
+ * bytes. No reference counterpart as such: the reference's cache is fp32,
+ * [layer][position][head][D] (src/qwen2_internal.h:34-42), which is one page
+ * per sequence here.
+ */
+#define QMV_TYPE_F32 0u
+#define QMV_TYPE_F16 1u
+#define QMV_TYPE_BF16 30u
+typedef struct QmvPagedCache {
+    void *keys;
+    void *values;
+    uint32_t type;
+    int kv_heads;
+    int head_dim; /* D: a multiple of 8 up to 128 */
+    int page_size;
+    int pages;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t token_stride;
+} QmvPagedCache;
+
+/*
+ * Rotary embedding of the new tokens' queries and keys
+ * (src/transformer_ops.cpp:43) and the write of keys and values into the cache,
+ * what the decode step does after the q/k/v projections. Token t's heads are rows of head_dim floats from d_q + t * q_stride,
+ * d_k + t * k_stride and d_v + t * v_stride (a stride of 0: the heads alone);
+ * d_q_out and d_k_out have the strides of d_q and d_k and may be them. Pair i <
+ * rotary_dims / 2 of a head at position p turns by the angle p *
+ * d_frequencies[i], a product in 64 bits: (x, y) becomes (x cos - y sin, x sin
+ * + y cos) with x, y the elements i and i + rotary_dims / 2, or 2 i and 2 i + 1
+ * with interleaved != 0. Elements from rotary_dims on are copied; rotary_dims
+ * is a multiple of 8 up to head_dim, 0 for none (d_frequencies may then be
+ * null).
+ * With a cache, k (turned) and v are stored at their positions, rounded to its
+ * type (nearest, ties to even; f16 overflows to infinity), and d_k_out may be
+ * null; cache may be null, and d_v then too. A position whose page is outside
+ * the cache or the table is not stored; d_status[0] is then set to 0, and left
+ * as it was otherwise (d_status may be null). Tokens at negative positions
+ * (more new tokens than the length says) are turned and not stored. Two tokens
+ * of a call that are stored in one place leave either.
+ * Pointers to floats are aligned to 16 bytes and strides are multiples of 4.
+ */
+int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q_heads,
+                               const float *d_k, int64_t k_stride,
+                               const float *d_v, int64_t v_stride,
+                               int kv_heads, int head_dim, int tokens,
+                               const double *d_frequencies, int rotary_dims,
+                               int interleaved, const QmvSequences *sequences,
+                               float *d_q_out, float *d_k_out,
+                               const QmvPagedCache *cache, int *d_status,
+                               void *stream);
+
+/*
+ * Causal attention over whole prompts, packed one after the other: token i of
+ * a sequence attends tokens 0 .. i of it, for each of q_heads heads (a
+ * multiple of kv_heads; head h reads key head h / (q_heads / kv_heads), the
+ * grouped attention of src/transformer_ops.cpp:71):
+ *   d_out[i] = sum_j softmax_j(scale * q_i . k_j) v_j
+ * Rows as above (strides, alignment); sequences' lengths and pages are not
+ * read. scale is finite. d_out overlaps no input.
+ */
+int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride,
+                                    const float *d_k, int64_t k_stride,
+                                    const float *d_v, int64_t v_stride,
+                                    int tokens, int q_heads, int kv_heads,
+                                    int head_dim, float scale,
+                                    const QmvSequences *sequences,
+                                    float *d_out, int64_t out_stride,
+                                    void *stream);
+
+/*
+ * The same for the new tokens of sequences whose keys and values, theirs
+ * included, are in a paged cache (written by qmv_device_rope_append_f32, say):
+ * the token at position p attends positions 0 .. p. One token per sequence is
+ * a decode step; several are a part of a prompt. A token at a negative position
+ * attends nothing and gets zeros. Where a page that a token attends is outside
+ * the cache or the table its row is NaN and d_status[0] is set to 0, else left
+ * as it was (d_status may be null). What lies in the cache behind a sequence's
+ * length is never used.
+ *
+ * Both forms hold q, k and v to 22 bits or more and sum in fp32. A key or value
+ * that is not finite makes the rows that attend it not finite where it counts,
+ * and no others. The work of few tokens is cut along the length and joined in
+ * a fixed order, in a workspace of the stream, so a capture needs one call of
+ * its size before it (see qmv_device_matvec_f32).
+ */
+int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride,
+                                   int tokens, int q_heads, float scale,
+                                   const QmvSequences *sequences,
+                                   const QmvPagedCache *cache, float *d_out,
+                                   int64_t out_stride, int *d_status,
+                                   void *stream);
+
 /* ---- Library state ------------------------------------------------------ */
 
 /* Message describing the calling thread's most recent failure ("" if none). */

@@ -33,6 +33,10 @@ GGML_TYPE_Q6_K = 14
 BLOCK_ELEMENTS = {GGML_TYPE_Q5_0: 32, GGML_TYPE_Q8_0: 32, GGML_TYPE_Q4_K: 256, GGML_TYPE_Q6_K: 256}
 BLOCK_BYTES = {GGML_TYPE_Q5_0: 22, GGML_TYPE_Q8_0: 34, GGML_TYPE_Q4_K: 144, GGML_TYPE_Q6_K: 210}
 TYPE_NAMES = {GGML_TYPE_Q5_0: "Q5_0", GGML_TYPE_Q8_0: "Q8_0", GGML_TYPE_Q4_K: "Q4_K", GGML_TYPE_Q6_K: "Q6_K"}
+# Types of a paged cache, GGML codes as above.
+GGML_TYPE_F32 = 0
+GGML_TYPE_F16 = 1
+GGML_TYPE_BF16 = 30
 MAX_BATCH = 32  # QMV_MAX_BATCH: positions per device call (host calls take any batch)
 MAX_GROUP = 8
 
@@ -73,6 +77,39 @@ def make_view(buf: np.ndarray, ggml_type: int, rows: int, cols: int, offset: int
     return v
 
 
+class QmvSequences(ctypes.Structure):
+    """The tokens of a step (include/qmv_hip.h): addresses of device arrays."""
+
+    _fields_ = [("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("count", ctypes.c_int), ("table_stride", ctypes.c_int)]
+
+
+class QmvPagedCache(ctypes.Structure):
+    """Keys and values of one layer in pages (include/qmv_hip.h)."""
+
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("type", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("pages", ctypes.c_int), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64)]
+
+
+def make_sequences(d_starts: int, count: int, d_lengths: int = 0, d_pages: int = 0,
+                   table_stride: int = 0) -> QmvSequences:
+    """``count`` sequences by device addresses: starts int32 [count + 1], lengths
+    int32 [count], page numbers int32 [count, table_stride]."""
+    return QmvSequences(d_starts or None, d_lengths or None, d_pages or None, count, table_stride)
+
+
+def make_paged_cache(d_keys: int, d_values: int, ggml_type: int, kv_heads: int, head_dim: int, page_size: int,
+                     pages: int, page_stride: int = 0, head_stride: int = 0, token_stride: int = 0) -> QmvPagedCache:
+    """A cache by device addresses; strides in elements, 0: pages of
+    [kv_heads][page_size][head_dim]."""
+    token = token_stride or head_dim
+    head = head_stride or page_size * token
+    return QmvPagedCache(d_keys or None, d_values or None, ggml_type, kv_heads, head_dim, page_size, pages,
+                         page_stride or kv_heads * head, head, token)
+
+
 def packed_bytes(ggml_type: int, rows: int, cols: int) -> int:
     return rows * (cols // BLOCK_ELEMENTS[ggml_type]) * BLOCK_BYTES[ggml_type]
 
@@ -80,6 +117,9 @@ def packed_bytes(ggml_type: int, rows: int, cols: int) -> int:
 _fp = ctypes.POINTER(ctypes.c_float)
 _vp = ctypes.c_void_p
 _view_p = ctypes.POINTER(QmvTensorView)
+_seq_p = ctypes.POINTER(QmvSequences)
+_cache_p = ctypes.POINTER(QmvPagedCache)
+_ld = ctypes.c_int64
 
 # name -> (restype, argtypes); mirrors include/qmv_hip.h
 HIP_SIGNATURES = {
@@ -124,6 +164,14 @@ HIP_SIGNATURES = {
                                                                 _vp, _vp]),
     "qmv_device_rms_norm_matvec_swiglu_f32": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_float, ctypes.c_int, _vp,
                                                              _vp, _vp]),
+    "qmv_device_rope_append_f32": (ctypes.c_int, [_vp, _ld, ctypes.c_int, _vp, _ld, _vp, _ld, ctypes.c_int, ctypes.c_int,
+                                                  ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int, _seq_p, _vp, _vp,
+                                                  _cache_p, _vp, _vp]),
+    "qmv_device_attention_prompt_f32": (ctypes.c_int, [_vp, _ld, _vp, _ld, _vp, _ld, ctypes.c_int, ctypes.c_int,
+                                                       ctypes.c_int, ctypes.c_int, ctypes.c_float, _seq_p, _vp, _ld,
+                                                       _vp]),
+    "qmv_device_attention_paged_f32": (ctypes.c_int, [_vp, _ld, ctypes.c_int, ctypes.c_int, ctypes.c_float, _seq_p,
+                                                      _cache_p, _vp, _ld, _vp, _vp]),
 }
 
 SYNTH_SIGNATURES = {
@@ -392,6 +440,39 @@ def device_embed_rows(tensor: "DeviceTensor", d_ids: int, count: int, d_out: int
 
 def device_greedy_argmax(d_logits: int, vocab: int, d_result: int, stream: int = 0) -> None:
     if not hip_lib().qmv_device_greedy_argmax_f32(d_logits, vocab, d_result, stream):
+        raise QmvError(last_error())
+
+
+def device_rope_append(d_q: int, q_heads: int, d_k: int, d_v: int, kv_heads: int, head_dim: int, tokens: int,
+                       d_frequencies: int, rotary_dims: int, sequences: QmvSequences, d_q_out: int, d_k_out: int = 0,
+                       cache: Optional[QmvPagedCache] = None, interleaved: bool = False, d_status: int = 0,
+                       stream: int = 0, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0) -> None:
+    """Rotary embedding of q and k at their positions into d_q_out and d_k_out
+    (which may be d_q and d_k), and k and v into the cache's pages."""
+    if not hip_lib().qmv_device_rope_append_f32(d_q, q_stride, q_heads, d_k, k_stride, d_v or None, v_stride, kv_heads,
+                                                head_dim, tokens, d_frequencies or None, rotary_dims,
+                                                1 if interleaved else 0, ctypes.byref(sequences), d_q_out,
+                                                d_k_out or None, ctypes.byref(cache) if cache is not None else None,
+                                                d_status or None, stream):
+        raise QmvError(last_error())
+
+
+def device_attention_prompt(d_q: int, d_k: int, d_v: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int,
+                            scale: float, sequences: QmvSequences, d_out: int, stream: int = 0, q_stride: int = 0,
+                            k_stride: int = 0, v_stride: int = 0, out_stride: int = 0) -> None:
+    """Causal attention over whole prompts packed one after the other."""
+    if not hip_lib().qmv_device_attention_prompt_f32(d_q, q_stride, d_k, k_stride, d_v, v_stride, tokens, q_heads,
+                                                     kv_heads, head_dim, scale, ctypes.byref(sequences), d_out,
+                                                     out_stride, stream):
+        raise QmvError(last_error())
+
+
+def device_attention_paged(d_q: int, tokens: int, q_heads: int, scale: float, sequences: QmvSequences,
+                           cache: QmvPagedCache, d_out: int, stream: int = 0, q_stride: int = 0, out_stride: int = 0,
+                           d_status: int = 0) -> None:
+    """Attention of the sequences' new tokens over their paged cache."""
+    if not hip_lib().qmv_device_attention_paged_f32(d_q, q_stride, tokens, q_heads, scale, ctypes.byref(sequences),
+                                                    ctypes.byref(cache), d_out, out_stride, d_status or None, stream):
         raise QmvError(last_error())
 
 

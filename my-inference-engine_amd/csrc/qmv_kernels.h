@@ -148,6 +148,45 @@ struct BatchParams {
     double *ssq;     /* with norm_w, launches that are not fused: [units][position slots] */
 };
 
+/* The tokens of a step and where their keys and values are (QmvSequences and
+ * QmvPagedCache of the C ABI, or a prompt's own rows). Strides in elements. */
+struct AttnTokens {
+    const int *starts, *lengths, *table;
+    int count, table_stride;
+    int tokens;    /* rows of q and out */
+    int heads, kv_heads, dim;
+    int page_size; /* 0: no pages, key j of a sequence is row start + j */
+    int pages;
+    int64_t page_stride, head_stride, token_stride;
+    int *status; /* may be null */
+};
+
+struct AttnParams {
+    AttnTokens t;
+    const float *q;
+    const void *k, *v;
+    float *out;
+    int64_t q_stride, out_stride;
+    float scale;
+};
+
+struct RopeParams {
+    AttnTokens t; /* the cache; page_size 0: none */
+    const float *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride; /* outputs as their inputs */
+    const double *freq;
+    int rotary, interleaved;
+    float *q_out, *k_out; /* k_out may be null */
+    void *keys, *values;
+};
+
+/* Types of keys and values. */
+#define QMV_KV_F32 0
+#define QMV_KV_F16 1
+#define QMV_KV_BF16 2
+hipError_t launch_attention(const AttnParams &p, int type, hipStream_t s);
+hipError_t launch_rope(const RopeParams &p, int type, hipStream_t s);
+
 /* Row-major epilogues. */
 #define QMV_ROWDOT_STORE 0
 #define QMV_ROWDOT_SWIGLU 1

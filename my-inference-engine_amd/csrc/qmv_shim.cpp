@@ -37,6 +37,7 @@
 #include "qmv_hip.h"
 #include "qmv_kernels.h"
 #include "qmv_layout.h"
+#include "qmv_shim.h"
 
 #define QMV_API extern "C" __attribute__((visibility("default")))
 
@@ -2310,6 +2311,27 @@ QMV_API int qmv_device_dequantize_f32(qmv_device_tensor t, int first_row, int ro
                                 (hipStream_t)stream));
     return 1;
 }
+
+/* ---- what the attention entry points share with these (qmv_shim.h) ---------- */
+
+namespace qmv {
+
+void shim_error(const char *text)
+{
+    t_error = text;
+}
+
+int shim_device()
+{
+    return g_device.load();
+}
+
+hipError_t shim_malloc(void **p, size_t bytes)
+{
+    return counted_malloc(p, bytes);
+}
+
+} // namespace qmv
 
 QMV_API const char *qmv_last_error(void)
 {

@@ -1,0 +1,520 @@
+"""Attention over packed prompts and over a paged cache, and rotary embedding
+with the cache write, against 64 bits (tests/_attention.py derives the
+bounds)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import _attention as A
+import _blocks as B
+
+pytestmark = pytest.mark.gpu
+
+MARK = np.float32(-12345.0)
+
+
+def log(msg):
+    print(msg, flush=True)
+
+
+@pytest.fixture(scope="module")
+def hip(qmv, gpu):
+    return A.hip_module()
+
+
+def _rand(rng, *shape, wide=1.0):
+    x = rng.standard_normal(shape)
+    return (x * np.where(rng.random(shape[-1]) < 0.1, wide, 1.0)).astype(np.float32)
+
+
+def _check(o, ref, bound, what):
+    err = np.abs(o.astype(np.float64) - ref)
+    assert np.isfinite(o).all(), f"{what}: not finite"
+    worst = np.max(err / np.maximum(bound, 1e-300))
+    log(f"{what}: error {np.max(err):.2e}, {worst:.3f} of the bound")
+    assert worst <= 1.0, what
+
+
+def _prompt(qmv, hip, new, heads, kv_heads, dim, q, k, v, scale, extra=(0, 0, 0), tail=0, stream=0, starts=None):
+    """The output [T + tail, heads, dim], rows of `tail` tokens no sequence has
+    among them; every row's gap is checked to stay as it was."""
+    T = q.shape[0]
+    ws, wk = heads * dim, kv_heads * dim
+    qs, ks, os_ = ws + extra[0], wk + extra[1], ws + extra[2]
+    dq = hip.DeviceBuffer.from_array(A.pack(q.reshape(T, ws), qs, ws))
+    dk, dv = (hip.DeviceBuffer.from_array(A.pack(x.reshape(T, wk), ks, wk)) for x in (k, v))
+    do = hip.DeviceBuffer.from_array(np.full((T, os_), MARK, np.float32))
+    if starts is None:
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    ds = hip.DeviceBuffer.from_array(starts)
+    seq = qmv.make_sequences(ds.ptr, len(starts) - 1)
+    qmv.device_attention_prompt(dq.ptr, dk.ptr, dv.ptr, T, heads, kv_heads, dim, scale, seq, do.ptr, stream, qs, ks, ks, os_)
+    hip.synchronize()
+    out = do.to_array(np.float32, (T, os_))
+    assert (out[:, ws:] == MARK).all()
+    return out[:, :ws].reshape(T, heads, dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(14, 2, 64), (12, 2, 128), (28, 4, 128), (3, 3, 8), (8, 1, 40), (5, 5, 96),
+                                                (16, 2, 120), (33, 1, 16)])
+@pytest.mark.parametrize("new", [[1], [37], [0, 1, 65, 0, 2, 130, 17]])
+def test_prompt(qmv, hip, heads, kv_heads, dim, new):
+    rng = np.random.default_rng(1000 * heads + dim)
+    T = sum(new)
+    q, k, v = _rand(rng, T, heads, dim, wide=2), _rand(rng, T, kv_heads, dim, wide=3), _rand(rng, T, kv_heads, dim)
+    scale = dim ** -0.5
+    o = _prompt(qmv, hip, new, heads, kv_heads, dim, q, k, v, scale, extra=(8, 4, 12))
+    t = 0
+    for s, n in enumerate(new):
+        if n:
+            ref, bound = A.attention64(q[t:t + n], k[t:t + n], v[t:t + n], scale, range(n))
+            _check(o[t:t + n], ref, bound, f"prompt {heads}/{kv_heads}/{dim} sequence {s} of {n}")
+        t += n
+
+
+@pytest.mark.parametrize("n", [300, 515])
+def test_prompt_long(qmv, hip, n):
+    rng = np.random.default_rng(n)
+    heads, kv_heads, dim = 4, 2, 128
+    q, k, v = _rand(rng, n, heads, dim, wide=2), _rand(rng, n, kv_heads, dim, wide=3), _rand(rng, n, kv_heads, dim)
+    o = _prompt(qmv, hip, [n], heads, kv_heads, dim, q, k, v, dim ** -0.5)
+    ref, bound = A.attention64(q, k, v, dim ** -0.5, range(n))
+    _check(o, ref, bound, f"prompt of {n}")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_prompt_scales(qmv, hip, scale):
+    rng = np.random.default_rng(3)
+    q, k, v = _rand(rng, 70, 2, 64), _rand(rng, 70, 1, 64), _rand(rng, 70, 1, 64)
+    o = _prompt(qmv, hip, [70], 2, 1, 64, q, k, v, scale)
+    ref, bound = A.attention64(q, k, v, scale, range(70))
+    _check(o, ref, bound, f"scale {scale}")
+
+
+def test_prompt_leaves_rows_of_no_sequence(qmv, hip):
+    """Tokens before the first start, behind the last and between none."""
+    rng = np.random.default_rng(4)
+    q, k, v = _rand(rng, 50, 4, 64), _rand(rng, 50, 2, 64), _rand(rng, 50, 2, 64)
+    o = _prompt(qmv, hip, None, 4, 2, 64, q, k, v, 0.125, starts=np.array([3, 3, 20, 41, 41], np.int32))
+    assert (o[:3] == MARK).all() and (o[41:] == MARK).all()
+    for a, b in ((3, 20), (20, 41)):
+        ref, bound = A.attention64(q[a:b], k[a:b], v[a:b], 0.125, range(b - a))
+        _check(o[a:b], ref, bound, f"rows {a}..{b}")
+
+
+def test_prompt_cuts_starts_to_the_tokens(qmv, hip):
+    """Starts that leave the call's tokens, or fall, write nothing outside it."""
+    rng = np.random.default_rng(5)
+    q, k, v = _rand(rng, 40, 2, 64), _rand(rng, 40, 2, 64), _rand(rng, 40, 2, 64)
+    o = _prompt(qmv, hip, None, 2, 2, 64, q, k, v, 0.125, starts=np.array([0, 30, 1000000], np.int32))
+    ref, bound = A.attention64(q[:30], k[:30], v[:30], 0.125, range(30))
+    _check(o[:30], ref, bound, "before the cut")
+    ref, bound = A.attention64(q[30:], k[30:], v[30:], 0.125, range(10))
+    _check(o[30:], ref, bound, "cut")
+
+
+@pytest.mark.parametrize("magnitude", [1e-30, 1e-6, 3e4, 1e18, 1e36])
+def test_prompt_magnitudes(qmv, hip, magnitude):
+    """Values, and keys against queries, far from one; rows of other sizes in
+    one tile."""
+    rng = np.random.default_rng(6)
+    q, k, v = _rand(rng, 90, 2, 64), _rand(rng, 90, 1, 64), _rand(rng, 90, 1, 64)
+    m = np.float32(magnitude)
+    o = _prompt(qmv, hip, [90], 2, 1, 64, q / m, k * m, v * m, 0.125)
+    ref, bound = A.attention64(q / m, k * m, v * m, 0.125, range(90))
+    _check(o, ref, bound, f"magnitude {magnitude}")
+    grow = (2.0 ** np.linspace(-20, 20, 90)).astype(np.float32)[:, None, None]
+    o = _prompt(qmv, hip, [90], 2, 1, 64, q, k, v * grow, 0.125)
+    ref, bound = A.attention64(q, k, v * grow, 0.125, range(90))
+    _check(o, ref, bound, "values that grow by the token")
+
+
+def test_prompt_not_finite(qmv, hip):
+    """A key or value that is not finite reaches the tokens that attend it and
+    no others, nor other heads; a query only its own row."""
+    rng = np.random.default_rng(7)
+    for bad in (np.inf, -np.inf, np.nan):
+        q, k, v = _rand(rng, 100, 4, 64), _rand(rng, 100, 2, 64), _rand(rng, 100, 2, 64)
+        v[40, 0, 5] = bad
+        k[70, 1, 3] = np.nan
+        q[10, 3, 0] = bad
+        o = _prompt(qmv, hip, [100], 4, 2, 64, q, k, v, 0.125)
+        assert not np.isfinite(o[40:, :2, 5]).any()
+        assert np.isnan(o[70:, 2:]).all()
+        assert not np.isfinite(o[10, 3]).any()
+        clean = np.ones_like(o, bool)
+        clean[40:, :2, 5] = clean[70:, 2:] = clean[10, 3] = False
+        q[10, 3, 0] = v[40, 0, 5] = k[70, 1, 3] = 0
+        ref, bound = A.attention64(q, k, v, 0.125, range(100))
+        _check(np.where(clean, o, 0), np.where(clean, ref, 0), np.where(clean, bound, 1), f"around {bad}")
+
+
+def _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, page, layout="heads", seed=0, tail=0):
+    rng = np.random.default_rng(seed)
+    b = A.Batch(new, length, page, seed)
+    keys = [_rand(rng, max(0, n), kv_heads, dim, wide=3) for n in b.length]
+    values = [_rand(rng, max(0, n), kv_heads, dim) for n in b.length]
+    keys, values = ([A.decode(A.encode(x, t), t) for x in y] for y in (keys, values))
+    q = _rand(rng, b.tokens + tail, heads, dim, wide=2)
+    cache = A.Cache(qmv, hip, b, keys, values, t, layout)
+    return b, q, keys, values, cache
+
+
+def _paged(qmv, hip, b, q, cache, scale, q_extra=0, out_extra=0, stream=None):
+    T, heads, dim = q.shape
+    w = heads * dim
+    dq = hip.DeviceBuffer.from_array(A.pack(q.reshape(T, w), w + q_extra, w))
+    do = hip.DeviceBuffer.from_array(np.full((T, w + out_extra), MARK, np.float32))
+    status = hip.DeviceBuffer.from_array(np.array([1, 77], np.int32))
+    seq = b.upload(qmv, hip)
+    qmv.device_attention_paged(dq.ptr, T, heads, scale, seq, cache.c, do.ptr, stream.handle if stream else 0, w + q_extra,
+                               w + out_extra, status.ptr)
+    hip.synchronize()
+    out = do.to_array(np.float32, (T, w + out_extra))
+    assert (out[:, w:] == MARK).all()
+    ok = status.to_array(np.int32, 2)
+    assert ok[1] == 77
+    return out[:, :w].reshape(T, heads, dim), int(ok[0])
+
+
+def _check_paged(b, q, keys, values, o, scale, what):
+    for s, n in enumerate(b.new):
+        if n:
+            a = int(b.starts[s])
+            ref, bound = A.attention64(q[a:a + n], keys[s], values[s], scale, b.positions(s))
+            _check(o[a:a + n], ref, bound, f"{what} sequence {s} ({n} of {b.length[s]})")
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,layout", [
+    (14, 2, 64, 16, "heads"), (28, 4, 128, 64, "tokens"), (12, 2, 128, 1, "heads"), (6, 3, 40, 48, "wide"),
+    (33, 1, 96, 7, "shared"), (4, 4, 8, 256, "tokens")])
+@pytest.mark.parametrize("new,length", [([1], [1]), ([1, 1, 0, 1, 1], [300, 64, 0, 129, 2]), ([5, 1, 33, 8], [5, 77, 200, 65])])
+def test_paged(qmv, hip, t, heads, kv_heads, dim, page, layout, new, length):
+    b, q, keys, values, cache = _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, page, layout, seed=dim + page)
+    o, ok = _paged(qmv, hip, b, q, cache, dim ** -0.5, 4, 8)
+    assert ok == 1
+    _check_paged(b, q, keys, values, o, dim ** -0.5, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim} page {page} {layout}")
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("new,length", [([1], [2500]), ([3, 1], [1777, 1025]), ([40], [1400])])
+def test_paged_long(qmv, hip, t, new, length):
+    """Few rows over a long axis: the work is cut along it."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, new, length, 7, 1, 128, t, 32, seed=9)
+    o, ok = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
+    assert ok == 1
+    _check_paged(b, q, keys, values, o, 128 ** -0.5, f"{A.NAMES[t]} long")
+    again, _ = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
+    assert np.array_equal(o.view(np.uint32), again.view(np.uint32))
+
+
+def test_paged_rows_that_attend_nothing(qmv, hip):
+    """More new tokens than the length says: zeros at negative positions; idle
+    sequences; tokens behind the last sequence stay as they were."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [4, 0, 3, 2], [2, 5, 0, -3], 4, 2, 64, A.F16, 16, seed=11, tail=6)
+    o, ok = _paged(qmv, hip, b, q, cache, 0.125)
+    assert ok == 1
+    assert (o[:2] == 0).all() and (o[4:9] == 0).all() and (o[9:] == MARK).all()
+    ref, bound = A.attention64(q[2:4], keys[0], values[0], 0.125, [0, 1])
+    _check(o[2:4], ref, bound, "the two that stand somewhere")
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 30, None])
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+def test_paged_bad_pages(qmv, hip, bad, t):
+    """A page outside the cache, or a length outside the table: the rows that
+    attend it are NaN, others keep their values, and the status says so. No
+    address of such a page is read: the number is compared with the cache's
+    pages first (bounds that the kernel checks itself)."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [1, 40, 1], [200, 120, 50], 4, 2, 64, t, 16, seed=12)
+    if bad is None:
+        b.length[0] = b.columns * 16 + 500  # past the table
+        b.table[0, :] = b.table[0, 0]
+    else:
+        b.table[0, 3] = bad
+        b.table[1, 6] = bad  # positions 96..111, new tokens 16..31: 16.. attend it
+    o, ok = _paged(qmv, hip, b, q, cache, 0.125)
+    assert ok == 0
+    assert np.isnan(o[0]).all()
+    ref, bound = A.attention64(q[41:], keys[2], values[2], 0.125, b.positions(2))
+    _check(o[41:], ref, bound, "another sequence")
+    n = 40 if bad is None else 16
+    ref, bound = A.attention64(q[1:1 + n], keys[1], values[1], 0.125, b.positions(1)[:n])
+    _check(o[1:1 + n], ref, bound, "rows before the page")
+    assert bad is None or np.isnan(o[17:41]).all()
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+def test_paged_not_finite(qmv, hip, t):
+    """As test_prompt_not_finite, a chunk of new tokens over a cache."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [60], [150], 4, 2, 64, t, 16, seed=13)
+    for bad in (np.inf, np.nan):
+        k2, v2 = keys[0].copy(), values[0].copy()
+        v2[120, 0, 9] = bad  # new token 30
+        k2[130, 1, 0] = np.nan
+        c2 = A.Cache(qmv, hip, b, [k2], [v2], t)
+        o, _ = _paged(qmv, hip, b, q, c2, 0.125)
+        clean = np.ones_like(o, bool)
+        clean[30:, :2, 9] = clean[40:, 2:] = False
+        assert not np.isfinite(o[30:, :2, 9]).any() and np.isnan(o[40:, 2:]).all()
+        ref, bound = A.attention64(q, keys[0], values[0], 0.125, b.positions(0))
+        _check(np.where(clean, o, 0), np.where(clean, ref, 0), np.where(clean, bound, 1), f"{A.NAMES[t]} around {bad}")
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+def test_paged_magnitudes(qmv, hip, t):
+    rng = np.random.default_rng(14)
+    for m in (1e-4, 1e3) if t == A.F16 else (1e-30, 1e4, 1e30):
+        b = A.Batch([1, 20], [200, 100], 16, 1)
+        keys = [A.decode(A.encode(_rand(rng, n, 2, 64) * np.float32(m), t), t) for n in b.length]
+        values = [A.decode(A.encode(_rand(rng, n, 2, 64) * np.float32(m), t), t) for n in b.length]
+        q = _rand(rng, b.tokens, 4, 64) / np.float32(m)
+        cache = A.Cache(qmv, hip, b, keys, values, t)
+        o, ok = _paged(qmv, hip, b, q, cache, 0.125)
+        assert ok == 1
+        _check_paged(b, q, keys, values, o, 0.125, f"{A.NAMES[t]} magnitude {m}")
+
+
+def test_paged_shared_pages(qmv, hip):
+    """Sequences that begin alike read the same pages."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [1, 2, 1], [64, 64, 64], 4, 2, 64, A.F16, 16, seed=15)
+    b.table[1, :4] = b.table[0, :4]
+    b.table[2, :3] = b.table[0, :3]
+    keys[1], values[1] = keys[0], values[0]
+    for x in (keys, values):
+        x[2] = np.concatenate([x[0][:48], x[2][48:]])
+    o, ok = _paged(qmv, hip, b, q, cache, 0.125)
+    assert ok == 1
+    _check_paged(b, q, keys, values, o, 0.125, "shared pages")
+
+
+def test_paged_far_offsets(qmv, hip):
+    """Pages whose elements lie beyond 2^31 of the cache's first."""
+    dim, hk, page, stride = 64, 1, 16, (1 << 31) + 64
+    rng = np.random.default_rng(16)
+    k, v = (_rand(rng, 24, hk, dim).astype(np.float16) for _ in range(2))
+    bufs = [hip.DeviceBuffer(2 * (stride + page * dim)) for _ in range(2)]
+    for buf, a in zip(bufs, (k, v)):
+        full = np.zeros((2, page, dim), np.float16)
+        full.reshape(32, dim)[:24] = a[:, 0]
+        for p, at in ((0, stride), (1, 0)):  # the sequence's first page is the far one
+            part = np.ascontiguousarray(full[p])
+            hip.check(hip.rt().hipMemcpy(buf.ptr + 2 * at, part.ctypes.data, part.nbytes, hip.H2D))
+    b = A.Batch([2], [24], page)
+    b.table = np.array([[1, 0]], np.int32)
+    b.columns = 2
+    seq = b.upload(qmv, hip)
+    q = _rand(rng, 2, 2, dim)
+    dq, do = hip.DeviceBuffer.from_array(q), hip.DeviceBuffer(q.nbytes)
+    c = qmv.make_paged_cache(bufs[0].ptr, bufs[1].ptr, A.F16, hk, dim, page, 2, stride, page * dim, dim)
+    qmv.device_attention_paged(dq.ptr, 2, 2, 0.125, seq, c, do.ptr)
+    hip.synchronize()
+    ref, bound = A.attention64(q, k.astype(np.float32), v.astype(np.float32), 0.125, [22, 23])
+    _check(do.to_array(np.float32, q.shape), ref, bound, "far pages")
+
+
+def test_paged_graph_and_streams(qmv, hip):
+    """A captured call, replayed with other lengths and queries between eager
+    calls of the same stream; another stream at the same time."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [1, 1, 1], [900, 333, 1200], 14, 2, 64, A.F16, 16, seed=17)
+    scale = 0.125
+    dq, do = hip.DeviceBuffer.from_array(q), hip.DeviceBuffer(q.nbytes)
+    do2 = hip.DeviceBuffer(q.nbytes)
+    seq = b.upload(qmv, hip)
+    lengths = b.d[1]
+    with hip.Stream() as s, hip.Stream() as other:
+        qmv.device_attention_paged(dq.ptr, 3, 14, scale, seq, cache.c, do.ptr, s.handle)
+        s.synchronize()
+        _check_paged(b, q, keys, values, do.to_array(np.float32, q.shape), scale, "eager")
+        with hip.Graph(s) as g:
+            g.begin()
+            qmv.device_attention_paged(dq.ptr, 3, 14, scale, seq, cache.c, do.ptr, s.handle)
+            g.end()
+            for step, now in enumerate([[900, 333, 1200], [1, 300, 1199], [0, 64, 65], [700, 2, 1000]]):
+                b.length = now
+                lens = np.array(now, np.int32)
+                hip.check(hip.rt().hipMemcpy(lengths.ptr, lens.ctypes.data, lens.nbytes, hip.H2D))
+                do.fill(0xFF)
+                g.replay()
+                qmv.device_attention_paged(dq.ptr, 3, 14, scale, seq, cache.c, do2.ptr, other.handle)
+                s.synchronize()
+                other.synchronize()
+                o, o2 = do.to_array(np.float32, q.shape), do2.to_array(np.float32, q.shape)
+                assert np.array_equal(o.view(np.uint32), o2.view(np.uint32)), f"replay {step}"
+                for i in range(3):
+                    if now[i] == 0:
+                        assert (o[i] == 0).all()
+                    else:
+                        ref, bound = A.attention64(q[i:i + 1], keys[i], values[i], scale, [now[i] - 1])
+                        _check(o[i:i + 1], ref, bound, f"replay {step} sequence {i}")
+
+
+# ---- rotary embedding and the cache write ------------------------------------------
+
+def _rope_bound(x):
+    """The angle's rest is rounded to fp32 (at most 2^-22.3 absolute, see the
+    kernel), sine and cosine to 2 steps of fp32, products and their sum to half
+    a step each: under 2^-21 of |x| + |y|, whose largest is twice max |x|."""
+    return 2.0 ** -21 * 2 * np.max(np.abs(x)) + 2.0 ** -140
+
+
+@pytest.mark.parametrize("t", A.TYPES + [None], ids=lambda t: A.NAMES.get(t, "none"))
+@pytest.mark.parametrize("heads,kv_heads,dim,rotary,page,layout", [
+    (14, 2, 64, 64, 16, "heads"), (28, 4, 128, 128, 64, "tokens"), (3, 1, 40, 24, 1, "wide"), (5, 5, 8, 0, 7, "heads")])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_append(qmv, hip, t, heads, kv_heads, dim, rotary, page, layout, interleaved):
+    rng = np.random.default_rng(20 + dim)
+    b = A.Batch([1, 0, 5, 17, 2], [1000, 0, 5, 40, 1], page, 3)
+    T = b.tokens + 4
+    q, k, v = _rand(rng, T, heads, dim, wide=4), _rand(rng, T, kv_heads, dim, wide=4), _rand(rng, T, kv_heads, dim)
+    f = A.frequencies(rotary)
+    qs, ks = heads * dim + 4, kv_heads * dim + 8
+    dq, dk, dv = (hip.DeviceBuffer.from_array(A.pack(x.reshape(T, -1), st, w)) for x, st, w in
+                  ((q, qs, heads * dim), (k, ks, kv_heads * dim), (v, ks, kv_heads * dim)))
+    dqo, dko = (hip.DeviceBuffer.from_array(np.full((T, st), MARK, np.float32)) for st in (qs, ks))
+    df = hip.DeviceBuffer.from_array(f if rotary else np.zeros(1))
+    status = hip.DeviceBuffer.from_array(np.array([1], np.int32))
+    seq = b.upload(qmv, hip)
+    cache = None
+    if t is not None:
+        blank = [np.full((max(0, n), kv_heads, dim), np.nan, np.float32) for n in b.length]
+        cache = A.Cache(qmv, hip, b, blank, blank, t, layout)
+        before = [cache.read(0), cache.read(1)]
+    qmv.device_rope_append(dq.ptr, heads, dk.ptr, dv.ptr, kv_heads, dim, T, df.ptr if rotary else 0, rotary, seq, dqo.ptr,
+                           dko.ptr, cache.c if cache else None, interleaved, status.ptr, 0, qs, ks, ks)
+    hip.synchronize()
+    assert status.to_array(np.int32, 1)[0] == 1
+    qo, ko = dqo.to_array(np.float32, (T, qs)), dko.to_array(np.float32, (T, ks))
+    assert (qo[:, heads * dim:] == MARK).all() and (ko[:, kv_heads * dim:] == MARK).all()
+    assert (qo[b.tokens:] == MARK).all() and (ko[b.tokens:] == MARK).all()
+    for s, n in enumerate(b.new):
+        for i, pos in enumerate(b.positions(s)):
+            a = int(b.starts[s]) + i
+            for x, o, h in ((q[a], qo[a], heads), (k[a], ko[a], kv_heads)):
+                y = o[:h * dim].reshape(h, dim)
+                ref = A.rope64(x, pos, f, interleaved)
+                assert np.max(np.abs(y - ref)) <= _rope_bound(x), (s, i)
+                assert np.array_equal(y[:, rotary:], x[:, rotary:])
+            if cache is not None and pos >= 0:
+                for which, rows in ((0, ko[a, :kv_heads * dim].reshape(kv_heads, dim)), (1, v[a])):
+                    for h in range(kv_heads):
+                        before[which][cache.at(s, pos, h)] = A.encode(rows[h], t)
+    if cache is not None:
+        for which in (0, 1):
+            after = cache.read(which)
+            assert np.array_equal(after.view(np.uint8), before[which].view(np.uint8)), "codes, and all else as it was"
+
+
+@pytest.mark.parametrize("position", [0, 131071, 4000000, 2000000000])
+def test_rope_far_positions(qmv, hip, position):
+    rng = np.random.default_rng(21)
+    q, k = _rand(rng, 1, 2, 128), _rand(rng, 1, 1, 128)
+    f = A.frequencies(128)
+    dq, dk, df = (hip.DeviceBuffer.from_array(x) for x in (q, k, f))
+    ds = [hip.DeviceBuffer.from_array(np.array(x, np.int32)) for x in ([0, 1], [position + 1])]
+    seq = qmv.make_sequences(ds[0].ptr, 1, ds[1].ptr)
+    qmv.device_rope_append(dq.ptr, 2, dk.ptr, 0, 1, 128, 1, df.ptr, 128, seq, dq.ptr, dk.ptr)  # in place
+    hip.synchronize()
+    for d, x in ((dq, q), (dk, k)):
+        # the product position * frequency is rounded to 64 bits on both sides: 2^-53 of at most 2^31
+        assert np.max(np.abs(d.to_array(np.float32, x.shape)[0] - A.rope64(x[0], position, f, False))) <= _rope_bound(x) + 2.0 ** -21
+
+
+def test_rope_bad_pages(qmv, hip):
+    """Nothing is stored where the page is outside the cache or the table."""
+    for bad in (-1, 1 << 30, None):
+        b = A.Batch([2, 1, 1], [20, 9, 9], 16, 4)
+        blank = [np.full((n, 1, 64), np.nan, np.float32) for n in b.length]
+        cache = A.Cache(qmv, hip, b, blank, blank, A.F32)
+        before = [cache.read(0), cache.read(1)]
+        if bad is None:
+            b.length[0] = 16 * b.columns + 30
+        else:
+            b.table[0, 1] = bad
+        rng = np.random.default_rng(22)
+        q, k, v = _rand(rng, 4, 2, 64), _rand(rng, 4, 1, 64), _rand(rng, 4, 1, 64)
+        dq, dk, dv, df = (hip.DeviceBuffer.from_array(x) for x in (q, k, v, A.frequencies(64)))
+        status = hip.DeviceBuffer.from_array(np.array([1], np.int32))
+        seq = b.upload(qmv, hip)
+        qmv.device_rope_append(dq.ptr, 2, dk.ptr, dv.ptr, 1, 64, 4, df.ptr, 64, seq, dq.ptr, 0, cache.c, d_status=status.ptr)
+        hip.synchronize()
+        assert status.to_array(np.int32, 1)[0] == 0
+        for s in (1, 2):
+            a = int(b.starts[s])
+            before[1][cache.at(s, 8, 0)] = v[a, 0]
+            got = cache.read(0)[cache.at(s, 8, 0)]
+            assert np.max(np.abs(got - A.rope64(k[a], 8, A.frequencies(64), False)[0])) <= _rope_bound(k[a])
+            before[0][cache.at(s, 8, 0)] = got
+        for which in (0, 1):
+            assert np.array_equal(cache.read(which).view(np.uint32), before[which].view(np.uint32))
+
+
+# ---- a run of them together ----------------------------------------------------------
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+def test_attention_block_of_a_layer(qmv, oracle, hip, t):
+    """Norm and q|k|v projections, rotary embedding into the cache, attention
+    and the output projection with the residual: two sequences in chunks and
+    then token by token, against 64 bits from the rows the projections wrote;
+    the first chunks also as whole prompts."""
+    heads, kv_heads, dim, hidden, page = 14, 2, 64, 896, 16
+    shapes = [(hidden, hidden), (kv_heads * dim, hidden), (kv_heads * dim, hidden), (hidden, hidden)]
+    raws = [qmv.synth_tensor(B.Q8_0, r, c, seed=50 + i) for i, (r, c) in enumerate(shapes)]
+    wq, wk, wv, wo = (qmv.DeviceTensor(qmv.make_view(raw, B.Q8_0, r, c)) for raw, (r, c) in zip(raws, shapes))
+    rng = np.random.default_rng(30)
+    norm = hip.DeviceBuffer.from_array((1 + 0.1 * rng.standard_normal(hidden)).astype(np.float32))
+    f = A.frequencies(dim)
+    df = hip.DeviceBuffer.from_array(f)
+    full = [61, 40]  # the lengths at the end
+    whole = A.Batch([0, 0], full, page, 5)
+    blank = [np.zeros((n, kv_heads, dim), np.float32) for n in full]
+    cache = A.Cache(qmv, hip, whole, blank, blank, t)
+    keys, values = [np.zeros((0, kv_heads, dim), np.float32)] * 2, [np.zeros((0, kv_heads, dim), np.float32)] * 2
+    have = [0, 0]
+    for new in ([20, 12], [11, 0], [1, 1], [28, 1], [1, 0], [0, 26]):
+        for s in (0, 1):
+            have[s] += new[s]
+        step = A.Batch(new, list(have), page)
+        step.table, step.columns = whole.table, whole.columns
+        seq = step.upload(qmv, hip)
+        T = step.tokens
+        x = rng.standard_normal((T, hidden)).astype(np.float32)
+        dx = hip.DeviceBuffer.from_array(x)
+        dq, dk, dv, dn, datt = (hip.DeviceBuffer(4 * T * w) for w in (hidden, 128, 128, hidden, hidden))
+        qmv.device_rms_norm_matvec_add_group([wq, wk, wv], dx.ptr, norm.ptr, 1e-6, T, None, None, [dq.ptr, dk.ptr, dv.ptr],
+                                             dn.ptr)
+        hip.synchronize()
+        q, k, v = (d.to_array(np.float32, (T, h, dim)) for d, h in ((dq, heads), (dk, kv_heads), (dv, kv_heads)))
+        qmv.device_rope_append(dq.ptr, heads, dk.ptr, dv.ptr, kv_heads, dim, T, df.ptr, dim, seq, dq.ptr, dk.ptr, cache.c)
+        qmv.device_attention_paged(dq.ptr, T, heads, dim ** -0.5, seq, cache.c, datt.ptr)
+        hip.synchronize()
+        att = datt.to_array(np.float32, (T, heads, dim))
+        qr, kr = dq.to_array(np.float32, q.shape), dk.to_array(np.float32, k.shape)
+        for s in (0, 1):
+            a, e = int(step.starts[s]), int(step.starts[s + 1])
+            for i, pos in enumerate(step.positions(s)):
+                assert np.max(np.abs(qr[a + i] - A.rope64(q[a + i], pos, f, False))) <= _rope_bound(q[a + i])
+                assert np.max(np.abs(kr[a + i] - A.rope64(k[a + i], pos, f, False))) <= _rope_bound(k[a + i])
+            keys[s] = np.concatenate([keys[s], A.decode(A.encode(kr[a:e], t), t)])
+            values[s] = np.concatenate([values[s], A.decode(A.encode(v[a:e], t), t)])
+        _check_paged(step, qr, keys, values, att, dim ** -0.5, f"{A.NAMES[t]} step {new}")
+        if have == new:
+            dp = hip.DeviceBuffer(att.nbytes)
+            qmv.device_attention_prompt(dq.ptr, dk.ptr, dv.ptr, T, heads, kv_heads, dim, dim ** -0.5, seq, dp.ptr)
+            hip.synchronize()
+            p = dp.to_array(np.float32, att.shape)
+            for s in (0, 1):
+                a, e = int(step.starts[s]), int(step.starts[s + 1])
+                ref, bound = A.attention64(qr[a:e], kr[a:e], v[a:e], dim ** -0.5, range(e - a))
+                _check(p[a:e], ref, bound, f"as prompts, sequence {s}")
+        qmv.device_matvec_add_group([wo], datt.ptr, T, [dx.ptr], [hidden], [dx.ptr])
+        hip.synchronize()
+        y = dx.to_array(np.float32, x.shape)
+        for i in range(T):
+            ref = oracle.matvec(raws[3], B.Q8_0, hidden, hidden, att[i].reshape(-1))
+            _, absdot = oracle.row_stats(raws[3], B.Q8_0, hidden, hidden, att[i].reshape(-1))
+            assert (np.abs(y[i] - (ref.astype(np.float64) + x[i])) <= 1e-5 * absdot + 2.0 ** -24 * np.abs(y[i])).all()
+    for w in (wq, wk, wv, wo):
+        w.close()
