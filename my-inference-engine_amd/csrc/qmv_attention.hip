@@ -12,21 +12,12 @@ namespace qmv {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float from_bf16(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-
 /* Nearest, ties to even; NaN stays NaN. */
 __device__ __forceinline__ uint16_t to_bf16(float v)
 {
     const uint32_t u = __float_as_uint(v);
     if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)(u >> 16 | 0x40u);
     return (uint16_t)((u + 0x7fffu + (u >> 16 & 1u)) >> 16);
-}
-
-template <int TYPE> __device__ __forceinline__ float load_kv(const void *base, int64_t i)
-{
-    if (TYPE == QMV_KV_F32) return ((const float *)base)[i];
-    if (TYPE == QMV_KV_F16) return (float)((const _Float16 *)base)[i];
-    return from_bf16(((const uint16_t *)base)[i]);
 }
 
 template <int TYPE> __device__ __forceinline__ void store_kv(void *base, int64_t i, float v)
@@ -62,61 +53,672 @@ __device__ __forceinline__ int64_t key_at(const AttnTokens &a, int s, int start,
     return (int64_t)at * a.page_stride + (int64_t)h * a.head_stride + (int64_t)(j - page * a.page_size) * a.token_stride;
 }
 
-/* A wave per token and head: lanes over keys for the scores, over the head's
- * elements for the values; the running maximum and sum of the softmax. */
-template <int TYPE> __global__ __launch_bounds__(256) void attention_kernel(AttnParams p)
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+
+#define QMV_LDS __attribute__((address_space(3)))
+
+/* Barrier for data exchanged through LDS: waits for this wave's LDS
+ * operations, not for the global loads of the next tile. */
+__device__ __forceinline__ void lds_barrier()
 {
-    const AttnTokens &a = p.t;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)a.tokens * a.heads) return;
-    const int t = (int)(item / a.heads), head = (int)(item % a.heads), kvh = head / (a.heads / a.kv_heads);
-    const int s = sequence_of(a, t);
-    if (s < 0) return;
-    const int start = a.starts[s], n = min(a.starts[s + 1], a.tokens) - start;
-    const int pos = (a.lengths ? a.lengths[s] - n : 0) + t - start;
-    const float *q = p.q + (int64_t)t * p.q_stride + (int64_t)head * a.dim;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j0 = 0; j0 <= pos; j0 += 64) {
-        const int j = j0 + lane;
-        const int64_t at = j <= pos ? key_at(a, s, start, j, kvh) : 0;
-        if (at < 0 && a.status) *a.status = 0;
-        float score = 0.f;
-        if (j <= pos && at >= 0)
-            for (int d = 0; d < a.dim; ++d) score = fmaf(q[d], load_kv<TYPE>(p.k, at + d), score);
-        score = j > pos ? -INFINITY : at < 0 ? NAN : score * p.scale;
-        float top = score;
-        bool nan = score != score;
-        for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-        top = __any(nan) ? NAN : fmaxf(m, top);
-        const float fade = m == -INFINITY ? 0.f : __expf(m - top);
-        float w = j > pos ? 0.f : __expf(score - top);
-        m = top;
-        l *= fade;
-        o0 *= fade;
-        o1 *= fade;
-        const int keys = pos - j0 < 63 ? pos - j0 + 1 : 64;
-        for (int i = 0; i < keys; ++i) {
-            const float wi = __shfl(w, i);
-            const int64_t ai = __shfl(at, i);
-            l += wi;
-            if (ai < 0) continue;
-            if (lane < a.dim) o0 = fmaf(wi, load_kv<TYPE>(p.v, ai + lane), o0);
-            if (lane + 64 < a.dim) o1 = fmaf(wi, load_kv<TYPE>(p.v, ai + lane + 64), o1);
-        }
-    }
-    float *out = p.out + (int64_t)t * p.out_stride + (int64_t)head * a.dim;
-    if (lane < a.dim) out[lane] = pos < 0 ? 0.f : o0 / l;
-    if (lane + 64 < a.dim) out[lane + 64] = pos < 0 ? 0.f : o1 / l;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F); /* lgkmcnt(0) */
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-hipError_t launch_attention(const AttnParams &p, int type, hipStream_t s)
+/* The larger of this lane's and lane ^ 32's. */
+__device__ __forceinline__ float max_halves(float x)
 {
-    const int64_t items = (int64_t)p.t.tokens * p.t.heads;
-    const dim3 grid((unsigned)((items + 3) / 4));
-    if (type == QMV_KV_F32) attention_kernel<QMV_KV_F32><<<grid, 256, 0, s>>>(p);
-    else if (type == QMV_KV_F16) attention_kernel<QMV_KV_F16><<<grid, 256, 0, s>>>(p);
-    else attention_kernel<QMV_KV_BF16><<<grid, 256, 0, s>>>(p);
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float sum_halves(float x)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+/* The largest of the wave's unsigned values, in every lane. */
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+#define QMV_STEP(CTRL) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
+    QMV_STEP(0x111) /* row_shr 1, 2, 4, 8: lane 15 of each row has the row's */
+    QMV_STEP(0x112)
+    QMV_STEP(0x114)
+    QMV_STEP(0x118)
+    QMV_STEP(0x142) /* row_bcast 15, 31: lane 63 has all */
+    QMV_STEP(0x143)
+#undef QMV_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t v, int lane)
+{
+    const int lo = __shfl((int)(uint32_t)v, lane), hi = __shfl((int)(v >> 32), lane);
+    return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+
+/* Agent-scope stores and loads of what workgroups pass to each other. */
+__device__ __forceinline__ void store_shared(float *p, float a, float b)
+{
+    const f2_t v = {a, b};
+    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f2_t load_shared(const float *p)
+{
+    return __builtin_bit_cast(f2_t, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+/* ---- attention -----------------------------------------------------------------
+ *
+ * A workgroup takes a tile of 32 WR rows of one sequence and key head, a row
+ * being a new token and one of the group's query heads, so every key and value
+ * that it reads serves the whole group; and a range of keys. A wave holds 32
+ * rows; WK waves take turns along the keys. Per 32 keys it computes
+ *   S^T = K Q^T   (matrix rows: keys; columns: rows of the tile)
+ *   O^T += V^T P^T
+ * with 32x32x16 products: a lane has one row's scores in its registers, and the
+ * registers that S^T leaves are the operand that O^T's product takes, with no
+ * exchange between lanes, if V's keys are read in the same order. The running
+ * maximum and sum are a lane's own, its other half's apart.
+ *
+ * Numbers. Products are of f16 with fp32 sums. q (times scale and log2 e) and
+ * the weights are two f16 limbs each, x = hi + lo, after a power of two has
+ * brought a row's largest |q| to [2^14, 2^15) and the weights to at most 2^15:
+ * 22 bits, or 2^-39 of the largest. f16 keys and values are operands as they
+ * are; those of bf16 are one limb and of f32 two, scaled in blocks of 16
+ * tokens by a power of two in the same way. The product of two low limbs (2^-22
+ * of the whole) is left out. A block's scale of the keys is a factor of its
+ * scores; that of the values is added to the exponents of its weights, and
+ * taken out again where the weights are summed.
+ *
+ * The weights' reference r follows the running maximum only when that is more
+ * than 2^4 over it, so that most tiles leave O as it is. */
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNothing = -3.0e38f; /* r before any key */
+constexpr float kShift = 11.f;       /* weights are at most 2^(kShift + kSlack) */
+constexpr float kSlack = 4.f;
+
+/* 2^n as a float, -126 <= n <= 127. */
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }
+
+/* The n with |x| 2^n in [2^14, 2^15) for the bits of a finite |x|, at most
+ * `most`. */
+__device__ __forceinline__ int scale_of(uint32_t bits, int most) { return min(14 - ((int)(bits >> 23) - 127), most); }
+
+/* Eight values as two limbs. */
+__device__ __forceinline__ void limbs_of(const float *x, float by, h8_t *hi, h8_t *lo)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = x[i] * by;
+        const _Float16 h = (_Float16)v;
+        (*hi)[i] = h;
+        (*lo)[i] = (_Float16)(v - (float)h);
+    }
+}
+
+/* What lanes read for keys past the end (zeros), and for keys whose page is not
+ * there (NaN in every type: the rows that attend them become NaN). */
+__device__ const u4_t kNoPiece[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {~0u, ~0u, ~0u, ~0u}, {~0u, ~0u, ~0u, ~0u}};
+constexpr int64_t kPastEnd = -2, kNoPage = -1;
+
+struct AttnItem {
+    int s, start, n, len; /* the sequence, its first token, new tokens and length (cut to its pages) */
+    int first;            /* position of its first new token */
+    int tile, tile_at;    /* of its row tiles; among all sequences' */
+    int split, chunk;     /* keys [split * chunk, ...) */
+};
+
+/* The `item`-th piece of a key head's work, by one wave: the sequences' row
+ * tiles, each cut into pieces of `chunk` keys, one after the other. chunk is
+ * chosen here from all lengths, so every workgroup has the same. */
+template <int BM, int STEP>
+__device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lane, AttnItem *out)
+{
+    const AttnTokens &a = p.t;
+    const int group = a.heads / a.kv_heads;
+    const int64_t room = a.page_size ? (int64_t)a.table_stride * a.page_size : INT32_MAX;
+    int start = 0, n = 0, len = 0, first = 0, tiles = 0;
+    auto read = [&](int s) {
+        start = n = len = first = tiles = 0;
+        if (s >= a.count) return;
+        start = min(max(a.starts[s], 0), a.tokens);
+        n = max(min(a.starts[s + 1], a.tokens) - start, 0);
+        len = a.lengths ? max(a.lengths[s], 0) : n;
+        first = len - n;
+        if (len > room) len = (int)room + 1; /* one key past the table: its rows are NaN */
+        tiles = (int)(((int64_t)n * group + BM - 1) / BM);
+    };
+    int64_t work = 0, rows = 0;
+    for (int s0 = 0; s0 < a.count; s0 += 64) {
+        read(s0 + lane);
+        work += (int64_t)tiles * len;
+        rows += n;
+    }
+#pragma unroll
+    for (int i = 32; i; i >>= 1) {
+        work += shfl64(work, lane ^ i);
+        rows += shfl64(rows, lane ^ i);
+    }
+    if (rows > a.tokens) return false; /* starts that fall */
+    int64_t chunk = INT32_MAX / STEP * STEP;
+    if (p.target) {
+        const int64_t pieces = max(p.target / a.kv_heads, 1);
+        chunk = max((work + pieces - 1) / pieces, (int64_t)2 * STEP);
+        chunk = (chunk + STEP - 1) / STEP * STEP;
+    }
+    int before = 0, tiles_before = 0;
+    for (int s0 = 0; s0 < a.count; s0 += 64) {
+        if (a.count > 64) read(s0 + lane);
+        const int splits = max((int)((len + chunk - 1) / chunk), 1);
+        const int items = tiles * splits;
+        int sum = items, tsum = tiles;
+#pragma unroll
+        for (int i = 1; i < 64; i <<= 1) {
+            const int u = __shfl_up(sum, i), v = __shfl_up(tsum, i);
+            if (lane >= i) {
+                sum += u;
+                tsum += v;
+            }
+        }
+        const uint64_t hit = __ballot(before + sum > item);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            const int mine = item - before - (__shfl(sum, at) - __shfl(items, at));
+            const int sp = __shfl(splits, at);
+            out->s = s0 + at;
+            out->start = __shfl(start, at);
+            out->n = __shfl(n, at);
+            out->len = __shfl(len, at);
+            out->first = __shfl(first, at);
+            out->chunk = (int)chunk;
+            out->tile = mine / sp;
+            out->split = mine - out->tile * sp;
+            out->tile_at = tiles_before + __shfl(tsum, at) - __shfl(tiles, at) + out->tile;
+            return true;
+        }
+        before += __shfl(sum, 63);
+        tiles_before += __shfl(tsum, 63);
+    }
+    return false;
+}
+
+/* DP: head_dim padded to 64 or 128; WR waves along the rows, WK along the
+ * keys. */
+template <int TYPE, int DP, int WR, int WK> struct AttnShape {
+    static constexpr int NL = TYPE == QMV_KV_F32 ? 2 : 1;   /* limbs of keys and values */
+    static constexpr int KT = WR >= 4 ? 64 : 32;            /* keys a wave takes per tile */
+    static constexpr int NB = KT / 16;                      /* blocks of 16 keys */
+    static constexpr int UNITS = 2 * NB / WR;               /* blocks (of keys, of values) a wave loads */
+    static constexpr int SLOTS = DP / 32;                   /* pieces of 8 elements a lane loads per block */
+    static constexpr int MAT = KT * DP * 2;                 /* bytes of a limb of keys or of values */
+    static constexpr int TILE = 2 * NL * MAT;
+    static constexpr int ROWS = 32 * WR;
+    static constexpr int JOIN = WK > 1 ? WK * (32 * DP * 4) : 0; /* the waves' O, where they meet */
+    static constexpr int LDS = WK * TILE > JOIN ? WK * TILE : JOIN;
+    static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
+};
+
+template <int TYPE, int DP, int WR, int WK>
+__global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
+{
+    using S = AttnShape<TYPE, DP, WR, WK>;
+    constexpr int KT = S::KT, NB = S::NB, UNITS = S::UNITS, SLOTS = S::SLOTS, MAT = S::MAT, NL = S::NL;
+    constexpr int THREADS = 64 * WR * WK, STEPS = DP / 16, DB = DP / 32;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
+    __shared__ float scales[WK][2 * NB]; /* of the keys: factors; of the values: exponents */
+    __shared__ uint32_t not_finite[WK][NB];
+    __shared__ float joined[WK > 1 ? WK : 1][2][32];
+
+    const AttnTokens &a = p.t;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wk = wave / WR, half = lane >> 5, col = lane & 31;
+    const int group = a.heads / a.kv_heads, dim = a.dim;
+    const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+    AttnItem it;
+    if (!find_item<S::ROWS, KT * WK>(p, gridDim.x / a.kv_heads - 1 - item, lane, &it)) return;
+
+
+    /* the keys of this piece */
+    const int last_token = min(it.n - 1, (it.tile * S::ROWS + S::ROWS - 1) / group);
+    const int keys = max(min(it.first + last_token + 1, it.len), 0);
+    const int pieces = max((int)(((int64_t)keys + it.chunk - 1) / it.chunk), 1);
+    if (it.split >= pieces) return;
+    const int begin = it.split * it.chunk, end = min((int64_t)keys, (int64_t)begin + it.chunk);
+    const int unmasked = it.first + it.tile * S::ROWS / group; /* every row attends keys up to here */
+
+    /* this lane's row: q as two limbs, its 8 elements of each 16-wide step */
+    const int row = it.tile * S::ROWS + wr * 32 + col;
+    const int token = row / group, head = kvh * group + row % group;
+    const bool real = token < it.n;
+    const int pos = real ? it.first + token : -1;
+    h8_t qhi[STEPS], qlo[STEPS];
+    float q_back;
+    {
+        const float *q = p.q + (int64_t)(it.start + token) * p.q_stride + (int64_t)head * dim;
+        const float by = p.scale * kLog2e;
+        float x[STEPS][8];
+        uint32_t bits = 0;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            const int d = 16 * st + 8 * half;
+            f4_t u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+            if (real && d < dim) {
+                u = *(const f4_t *)(q + d);
+                v = *(const f4_t *)(q + d + 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[st][i] = (i < 4 ? u[i & 3] : v[i & 3]) * by;
+                const uint32_t m = __float_as_uint(x[st][i]) & 0x7fffffffu;
+                if (m < 0x7f800000u) bits = max(bits, m);
+            }
+        }
+        const auto both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+        const int n = scale_of(max((uint32_t)both[0], (uint32_t)both[1]), 126);
+        q_back = power_of_two(-n);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) limbs_of(x[st], power_of_two(n), &qhi[st], &qlo[st]);
+    }
+
+    /* ---- tiles: loads into registers, then as f16 limbs into LDS ---- */
+    unsigned char *const tile = lds + wk * S::TILE;
+    constexpr int PIECES = DP / 8, PER = 64 / PIECES; /* of a key; keys per slot */
+    const int piece = lane % PIECES, sub = lane / PIECES;
+    constexpr int OWN = WR == 1 ? KT : 16; /* keys whose places a wave looks up */
+    const int own_first = WR == 1 ? 0 : 16 * (wr % NB);
+
+    /* Where lane's key (own_first + lane % OWN) of the tile at k0 begins. */
+    auto place = [&](int k0) -> int64_t {
+        const int j = k0 + own_first + (lane & (OWN - 1));
+        if (j >= end) return kPastEnd;
+        const int64_t at = key_at(a, it.s, it.start, j, kvh);
+        if (at < 0 && a.status) *a.status = 0;
+        return at;
+    };
+    constexpr int RAW = TYPE == QMV_KV_F32 ? 2 : 1; /* 16-byte loads per piece */
+    u4_t raw[UNITS][SLOTS][RAW];
+    auto unit_block = [&](int u) { return WR == 1 ? u % NB : wr % NB; };
+    auto unit_values = [&](int u) { return WR == 1 ? u >= NB : UNITS == 1 ? wr >= NB : u == 1; };
+    auto load = [&](int64_t at) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const unsigned char *base = (const unsigned char *)(unit_values(u) ? p.v : p.k);
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                const int64_t from = shfl64(at, (WR == 1 ? 16 * unit_block(u) : 0) + i * PER + sub);
+                const unsigned char *src = base + (from + 8 * piece) * (TYPE == QMV_KV_F32 ? 4 : 2);
+                if (from < 0 || 8 * piece >= dim)
+                    src = (const unsigned char *)(kNoPiece + (from == kNoPage && !unit_values(u) && 8 * piece < dim ? 2 : 0));
+#pragma unroll
+                for (int r = 0; r < RAW; ++r) raw[u][i][r] = ((const u4_t *)src)[r];
+            }
+        }
+    };
+    auto store = [&](bool masked) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int b = unit_block(u);
+            const bool values = unit_values(u);
+            unsigned char *to = tile + (values ? NL * MAT : 0) + 16 * b * DP * 2;
+            uint32_t top = 0; /* the largest magnitude, bits of fp32 (f16, bf16: of two codes) */
+            int n = 0;
+            if (TYPE != QMV_KV_F16 || (values && masked)) {
+                constexpr uint32_t inf = TYPE == QMV_KV_F32 ? 0x7f800000u : TYPE == QMV_KV_F16 ? 0x7c00u : 0x7f80u;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+                    for (int r = 0; r < RAW; ++r)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t w = raw[u][i][r][e];
+                            if (TYPE == QMV_KV_F32) {
+                                const uint32_t m = w & 0x7fffffffu;
+                                odd |= m >= inf;
+                                top = max(top, m >= inf ? 0u : m);
+                            } else {
+                                const uint32_t m0 = w & 0x7fffu, m1 = w >> 16 & 0x7fffu;
+                                odd |= m0 >= inf || m1 >= inf;
+                                top = max(top, max(m0 >= inf ? 0u : m0, m1 >= inf ? 0u : m1));
+                            }
+                        }
+                if (values) {
+                    const bool any = __any(odd);
+                    if (lane == 0) not_finite[wk][b] = any;
+                }
+                if (TYPE != QMV_KV_F16) {
+                    top = wave_max(top);
+                    n = scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? 100 : 126);
+                    if (lane == 0) scales[wk][values ? NB + b : b] = values ? (float)-n : power_of_two(-n);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                const int r = i * PER + sub;
+                const int turn = DP == 128 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3);
+                unsigned char *at = to + r * DP * 2 + ((piece ^ turn) << 4);
+                if (TYPE == QMV_KV_F16) {
+                    *(u4_t *)at = raw[u][i][0];
+                } else if (TYPE == QMV_KV_BF16) {
+                    h8_t h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[2 * e] = (_Float16)(__uint_as_float(raw[u][i][0][e] << 16) * power_of_two(n));
+                        h[2 * e + 1] = (_Float16)(__uint_as_float(raw[u][i][0][e] & 0xffff0000u) * power_of_two(n));
+                    }
+                    *(h8_t *)at = h;
+                } else {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[u][i][e >> 2][e & 3]);
+                    h8_t hi, lo;
+                    limbs_of(x, power_of_two(n), &hi, &lo);
+                    *(h8_t *)at = hi;
+                    *(h8_t *)(at + MAT) = lo;
+                }
+            }
+        }
+    };
+
+    /* ---- a tile's products ---- */
+    f16_t o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f16_t{0};
+    float r = kNothing, l = 0.f;
+    const int turn_k = DP == 128 ? (col & 3) << 2 | (col >> 2 & 3) : (col >> 1 & 1) << 2 | (col >> 2 & 3);
+    const int k_at = col * DP * 2 + ((half ^ turn_k) << 4);
+    const int kk = (lane & 15) >> 2; /* this lane's key of four in a transposing load */
+    int v_at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int key = 8 * i + 4 * half + kk;
+        const int low = ((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ (2 * i + half);
+        v_at[i] = key * DP * 2 + ((DP == 128 ? kk << 2 : (kk >> 1) << 2) + low) * 16 + (lane & 1) * 8;
+    }
+    /* V^T of 16 keys and 32 elements: 8 keys of one element a lane, in the order
+     * in which the scores are in its registers. */
+    auto v_frag = [&](int limb, int step, int db) -> h8_t {
+        const unsigned char *base = tile + (NL + limb) * MAT + step * 16 * DP * 2;
+        typedef QMV_LDS s4_t *ptr;
+        const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[0] ^ db << 6)));
+        const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[1] ^ db << 6)));
+        const h4_t hx = __builtin_bit_cast(h4_t, x), hy = __builtin_bit_cast(h4_t, y);
+        return h8_t{hx[0], hx[1], hx[2], hx[3], hy[0], hy[1], hy[2], hy[3]};
+    };
+    auto compute = [&](int k0) {
+#pragma unroll
+        for (int sb = 0; sb < KT / 32; ++sb) {
+            f16_t c = {0};
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                const unsigned char *at = tile + 32 * sb * DP * 2 + (k_at ^ st << 5);
+                const h8_t hi = *(const h8_t *)at;
+                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[st], c, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[st], c, 0, 0, 0);
+                if (NL == 2) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8_t *)(at + MAT), qhi[st], c, 0, 0, 0);
+            }
+            const int first = k0 + 32 * sb + 4 * half; /* key of register 8 g + i: first + 16 g + 8 (i / 4) + i % 4 */
+            const bool masked = k0 + 32 * sb + 31 > unmasked;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (first + 8 * (i >> 2) + (i & 3) > pos) c[i] = -INFINITY;
+            }
+            float by[2], add[2], back[2];
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                if (TYPE == QMV_KV_F16) {
+                    by[g] = q_back;
+                    add[g] = 0.f;
+                } else {
+                    /* within the finite positive floats, so that a masked score stays -inf */
+                    by[g] = fminf(fmaxf(q_back * scales[wk][2 * sb + g], 1.1754944e-38f), 1.7014118e38f);
+                    add[g] = scales[wk][NB + 2 * sb + g];
+                    back[g] = __builtin_ldexpf(1.f, -20 - (int)add[g]); /* may be a denormal */
+                }
+                float m = c[8 * g];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) m = fmaxf(m, c[8 * g + i]);
+                top = fmaxf(top, fmaf(m, by[g], add[g]));
+            }
+            top = max_halves(top);
+            if (__any(top > r + kSlack)) {
+                const float to = top > r + kSlack ? top : r;
+                const float fade = __builtin_amdgcn_exp2f(r - to);
+                r = to;
+                l *= fade;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[i] *= fade;
+            }
+            h8_t phi[2], plo[2];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const float shift = add[g] - r + kShift;
+                float w[8], sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(fmaf(c[8 * g + i], by[g], shift));
+                    sum += w[i];
+                }
+                limbs_of(w, 1.f, &phi[g], &plo[g]);
+                l = TYPE == QMV_KV_F16 ? l + sum : fmaf(sum, back[g], l);
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int step = 2 * sb + g;
+                if (masked && not_finite[wk][step]) {
+                    /* A value that is not finite must not reach the rows that do
+                     * not attend it, and 0 * inf is NaN: its place is zero in the
+                     * product, and a product of marks finds the rows that do. */
+                    h8_t seen;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        seen[i] = (_Float16)(first + 16 * g + 8 * (i >> 2) + (i & 3) <= pos ? 1.f : 0.f);
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        h8_t v = v_frag(0, step, db), mark;
+                        h8_t v2 = NL == 2 ? v_frag(1, step, db) : v;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const _Float16 x = v[i];
+                            const bool odd = (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00;
+                            mark[i] = (_Float16)(odd ? 1.f : 0.f);
+                            if (odd) v[i] = v2[i] = (_Float16)0.f;
+                        }
+                        f16_t hits = {0};
+                        hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(mark, seen, hits, 0, 0, 0);
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
+                        if (NL == 2) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, phi[g], o[db], 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (hits[i] > 0.f) o[db][i] = NAN;
+                    }
+                } else {
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const h8_t v = v_frag(0, step, db);
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
+                        if (NL == 2)
+                            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(1, step, db), phi[g], o[db], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+
+    constexpr int STEP = KT * WK;
+    int k0 = begin + wk * KT;
+    int64_t next = place(k0);
+    if (begin < end) load(next);
+    next = place(k0 + STEP);
+    for (int at = begin; at < end; at += STEP, k0 += STEP) {
+        if (WR > 1) lds_barrier(); /* the last tile has been read */
+        store(k0 + KT - 1 > unmasked);
+        if (at + STEP < end) load(next);
+        next = place(k0 + 2 * STEP);
+        if (WR > 1) lds_barrier();
+        else asm volatile("" ::: "memory");
+        if (k0 < end) compute(k0);
+        if (WR == 1) asm volatile("" ::: "memory");
+    }
+    l = sum_halves(l);
+    constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
+    const int64_t slot = (int64_t)(gridDim.x / a.kv_heads - 1 - item) * a.kv_heads + kvh; /* of split 0: less split * kv_heads */
+    float *const part = p.partials + slot * S::PARTIAL;
+    auto out_of = [&](int row_in_tile) -> float * {
+        const int rr = it.tile * S::ROWS + row_in_tile, tk = rr / group;
+        return tk < it.n ? p.out + (int64_t)(it.start + tk) * p.out_stride + (int64_t)(kvh * group + rr % group) * dim : nullptr;
+    };
+
+    if (WK == 1) {
+        /* register 4 j + i of o[db]: element 32 db + 8 j + 4 half + i of this lane's row */
+        float *out = out_of(wr * 32 + col);
+        const bool none = l == 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 32 * db + 8 * j + 4 * half;
+                f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+                if (pieces == 1) {
+                    v = none ? f4_t{0, 0, 0, 0} : v * kDown / l;
+                    if (out != nullptr && d < dim) *(f4_t *)(out + d) = v;
+                } else {
+                    float *to = part + (wr * 32 + col) * DP + d;
+                    store_shared(to, v[0], v[1]);
+                    store_shared(to + 2, v[2], v[3]);
+                }
+            }
+        if (pieces > 1 && half == 0) store_shared(part + S::ROWS * DP + 2 * (wr * 32 + col), r, l);
+    } else {
+        /* the waves' results meet in LDS */
+        if (half == 0) {
+            joined[wk][0][col] = r;
+            joined[wk][1][col] = l;
+        }
+        lds_barrier(); /* tiles are done with, too */
+        float top = joined[0][0][col];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, joined[w][0][col]);
+        float *mine = (float *)lds + wk * 32 * DP;
+        const float fade = __builtin_amdgcn_exp2f(r - top);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d4 = 8 * db + 2 * j + half;
+                const f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+                *(f4_t *)(mine + col * DP + ((d4 ^ (col & 7)) << 2)) = v * fade;
+            }
+        lds_barrier();
+#pragma unroll
+        for (int e = tid; e < 32 * DP / 4; e += THREADS) {
+            const int rr = e / (DP / 4), d4 = e % (DP / 4);
+            float all = joined[0][0][rr], sum = 0.f;
+#pragma unroll
+            for (int w = 1; w < WK; ++w) all = fmaxf(all, joined[w][0][rr]);
+            f4_t v = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
+                v += *(const f4_t *)((const float *)lds + w * 32 * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
+            }
+            if (pieces == 1) {
+                float *out = out_of(rr);
+                v = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
+                if (out != nullptr && 4 * d4 < dim) *(f4_t *)(out + 4 * d4) = v;
+            } else {
+                float *to = part + rr * DP + 4 * d4;
+                store_shared(to, v[0], v[1]);
+                store_shared(to + 2, v[2], v[3]);
+                if (d4 == 0) store_shared(part + S::ROWS * DP + 2 * rr, all, sum);
+            }
+        }
+    }
+    if (pieces == 1) return;
+
+    /* The last of a row tile's pieces joins them, in their order. */
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    uint32_t *const seat = &not_finite[0][0];
+    unsigned *const counter = p.counters + (int64_t)it.tile_at * a.kv_heads + kvh;
+    if (tid == 0) *seat = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    lds_barrier();
+    if (*seat != (uint32_t)pieces - 1u) return;
+    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float *first_part = part - (int64_t)it.split * a.kv_heads * S::PARTIAL;
+    const int64_t apart = (int64_t)a.kv_heads * S::PARTIAL;
+    for (int e = tid; e < S::ROWS * DP / 4; e += THREADS) {
+        const int rr = e / (DP / 4), d4 = e % (DP / 4);
+        float *out = out_of(rr);
+        if (out == nullptr || 4 * d4 >= dim) continue;
+        const float *state = first_part + S::ROWS * DP + 2 * rr, *val = first_part + rr * DP + 4 * d4;
+        float all = kNothing, sum = 0.f;
+        for (int i = 0; i < pieces; ++i) all = fmaxf(all, load_shared(state + i * apart)[0]);
+        f4_t v = {0, 0, 0, 0};
+        for (int i = 0; i < pieces; ++i) {
+            const f2_t st = load_shared(state + i * apart);
+            const f2_t x = load_shared(val + i * apart), y = load_shared(val + i * apart + 2);
+            const float fade = __builtin_amdgcn_exp2f(st[0] - all);
+            sum = fmaf(st[1], fade, sum);
+            v += f4_t{x[0], x[1], y[0], y[1]} * fade;
+        }
+        *(f4_t *)(out + 4 * d4) = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
+    }
+}
+
+AttnPlan plan_attention(const AttnTokens &t)
+{
+    AttnPlan plan = {};
+    const int group = t.heads / t.kv_heads;
+    const int64_t rows = (int64_t)t.tokens * group, each = rows / t.count;
+    plan.rows = each <= 48 ? 32 : each <= 1024 ? 128 : 256;
+    const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
+    plan.tiles = (int)tiles;
+    plan.target = tiles * t.kv_heads < 2048 ? 512 : 0;
+    const int64_t items = tiles + (plan.target ? plan.target / t.kv_heads + 1 : 0);
+    plan.grid = items * t.kv_heads;
+    if (plan.target) {
+        const int dp = t.dim <= 64 ? 64 : 128;
+        plan.partials = (size_t)plan.grid * (plan.rows * (dp + 2));
+        plan.counters = (size_t)(tiles * t.kv_heads);
+    }
+    return plan;
+}
+
+template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+{
+    const dim3 grid((unsigned)plan.grid);
+    if (plan.rows == 32) attention_kernel<TYPE, DP, 1, 4><<<grid, 256, 0, s>>>(p);
+    else if (plan.rows == 128) attention_kernel<TYPE, DP, 4, 1><<<grid, 256, 0, s>>>(p);
+    else attention_kernel<TYPE, DP, 8, 1><<<grid, 512, 0, s>>>(p);
+}
+
+template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+{
+    if (p.t.dim <= 64) launch_rows<TYPE, 64>(p, plan, s);
+    else launch_rows<TYPE, 128>(p, plan, s);
+}
+
+hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s)
+{
+    if (type == QMV_KV_F32) launch_dim<QMV_KV_F32>(p, plan, s);
+    else if (type == QMV_KV_F16) launch_dim<QMV_KV_F16>(p, plan, s);
+    else launch_dim<QMV_KV_BF16>(p, plan, s);
     return hipGetLastError();
 }
 

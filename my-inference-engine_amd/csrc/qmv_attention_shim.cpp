@@ -10,6 +10,11 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <map>
+#include <memory>
+#include <mutex>
+#include <utility>
+#include <vector>
 
 #include "qmv_hip.h"
 #include "qmv_kernels.h"
@@ -82,6 +87,10 @@ bool heads_ok(int tokens, int q_heads, int kv_heads, int head_dim)
         set_error("invalid token or head counts (%d tokens, %d and %d heads)", tokens, q_heads, kv_heads);
         return false;
     }
+    if ((int64_t)tokens * q_heads > INT_MAX / 2) {
+        set_error("more than 2^30 rows of tokens and heads");
+        return false;
+    }
     if (head_dim < 8 || head_dim > 128 || head_dim % 8 != 0) {
         set_error("head_dim must be a multiple of 8 from 8 to 128 (got %d)", head_dim);
         return false;
@@ -116,7 +125,7 @@ bool cache_ok(const QmvPagedCache *c, const QmvSequences *q, int *type)
         set_error("invalid heads of the cache (%d of %d)", c->kv_heads, c->head_dim);
         return false;
     }
-    if (c->pages <= 0 || c->page_size <= 0 || (int64_t)q->table_stride * c->page_size > INT_MAX) {
+    if (c->pages <= 0 || c->page_size <= 0 || (int64_t)q->table_stride * c->page_size > 1 << 30) {
         set_error("invalid pages (%d of %d tokens, %d per sequence)", c->pages, c->page_size, q->table_stride);
         return false;
     }
@@ -164,6 +173,78 @@ qmv::AttnTokens attn_tokens(const QmvSequences &q, int tokens, int heads, int kv
         t.token_stride = c->token_stride;
     }
     return t;
+}
+
+/* What a stream's calls of few rows pass between workgroups. Buffers only grow,
+ * and one that is replaced is kept: a graph captured earlier on the stream may
+ * still use it (and every launch leaves its counters at zero). */
+struct Workspace {
+    float *partials = nullptr;
+    unsigned *counters = nullptr;
+    size_t partial_cap = 0, counter_cap = 0;
+    std::vector<void *> retired;
+    std::mutex mu;
+};
+
+std::mutex g_workspaces_mu;
+std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>> g_workspaces;
+
+Workspace &workspace_for(int device, hipStream_t stream)
+{
+    std::lock_guard<std::mutex> lock(g_workspaces_mu);
+    auto &slot = g_workspaces[{device, stream}];
+    if (!slot) slot.reset(new Workspace());
+    return *slot;
+}
+
+/* The workspace grown to a plan's need, its mutex held. New counters are cleared
+ * on the stream by a kernel. */
+int workspace_reserve(Workspace &ws, hipStream_t stream, size_t partials, size_t counters)
+{
+    if (partials <= ws.partial_cap && counters <= ws.counter_cap) return 1;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
+        set_error("workspace must grow during stream capture; run the call once before capturing");
+        return 0;
+    }
+    if (partials > ws.partial_cap) {
+        const size_t n = partials + partials / 4;
+        void *buf = nullptr;
+        HIP_TRY(qmv::shim_malloc(&buf, n * sizeof(float)));
+        if (ws.partials) ws.retired.push_back(ws.partials);
+        ws.partials = (float *)buf;
+        ws.partial_cap = n;
+    }
+    if (counters > ws.counter_cap) {
+        const size_t n = counters + counters / 4 + 1024;
+        void *buf = nullptr;
+        HIP_TRY(qmv::shim_malloc(&buf, n * sizeof(unsigned)));
+        if (ws.counters) ws.retired.push_back(ws.counters);
+        ws.counters = (unsigned *)buf;
+        ws.counter_cap = 0;
+        HIP_TRY(qmv::launch_fill_u32(ws.counters, n, 0u, stream));
+        ws.counter_cap = n;
+    }
+    return 1;
+}
+
+int attend(qmv::AttnParams &p, int type, hipStream_t stream)
+{
+    const int device = qmv::shim_device();
+    HIP_TRY(hipSetDevice(device));
+    const qmv::AttnPlan plan = qmv::plan_attention(p.t);
+    if (plan.grid > INT_MAX) {
+        set_error("too many tokens and heads for one call");
+        return 0;
+    }
+    Workspace &ws = workspace_for(device, stream);
+    std::lock_guard<std::mutex> lock(ws.mu);
+    if (!workspace_reserve(ws, stream, plan.partials, plan.counters)) return 0;
+    p.target = plan.target;
+    p.partials = ws.partials;
+    p.counters = ws.counters;
+    HIP_TRY(qmv::launch_attention(p, plan, type, stream));
+    return 1;
 }
 
 } // namespace
@@ -270,7 +351,6 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
         set_error("k and v must have one stride");
         return 0;
     }
-    HIP_TRY(hipSetDevice(qmv::shim_device()));
     qmv::AttnParams p = {};
     p.t = attn_tokens(*sequences, tokens, q_heads, kv_heads, head_dim, nullptr, nullptr);
     p.t.lengths = nullptr;
@@ -284,8 +364,7 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.scale = scale;
-    HIP_TRY(qmv::launch_attention(p, QMV_KV_F32, (hipStream_t)stream));
-    return 1;
+    return attend(p, QMV_KV_F32, (hipStream_t)stream);
 }
 
 QMV_API int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride, int tokens, int q_heads, float scale,
@@ -314,7 +393,6 @@ QMV_API int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride, i
         set_error("the attention output overlaps q or the cache");
         return 0;
     }
-    HIP_TRY(hipSetDevice(qmv::shim_device()));
     qmv::AttnParams p = {};
     p.t = attn_tokens(*sequences, tokens, q_heads, kv_heads, head_dim, cache, d_status);
     p.q = d_q;
@@ -324,6 +402,5 @@ QMV_API int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride, i
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.scale = scale;
-    HIP_TRY(qmv::launch_attention(p, type, (hipStream_t)stream));
-    return 1;
+    return attend(p, type, (hipStream_t)stream);
 }

@@ -168,6 +168,21 @@ struct AttnParams {
     float *out;
     int64_t q_stride, out_stride;
     float scale;
+    /* Work of few rows is cut along the keys into about `target` pieces (0:
+     * not), whose partial results meet in the workspace. */
+    int target;
+    float *partials;    /* attn_partial_floats() for each workgroup */
+    unsigned *counters; /* one per row tile and key head, zero between launches */
+};
+
+/* How a call is launched: rows (token, head of the group) per workgroup, the
+ * workgroups and the workspace. */
+struct AttnPlan {
+    int rows;
+    int target;
+    int tiles; /* row tiles at most, of one key head */
+    int64_t grid;
+    size_t partials, counters; /* floats, words */
 };
 
 struct RopeParams {
@@ -184,7 +199,8 @@ struct RopeParams {
 #define QMV_KV_F32 0
 #define QMV_KV_F16 1
 #define QMV_KV_BF16 2
-hipError_t launch_attention(const AttnParams &p, int type, hipStream_t s);
+AttnPlan plan_attention(const AttnTokens &t);
+hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s);
 hipError_t launch_rope(const RopeParams &p, int type, hipStream_t s);
 
 /* Row-major epilogues. */
