@@ -277,7 +277,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     constexpr int THREADS = 64 * WR * WK, STEPS = DP / 16, DB = DP / 32;
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
     __shared__ float scales[WK][2 * NB]; /* of the keys: factors; of the values: exponents */
-    __shared__ uint32_t not_finite[WK][NB];
+    __shared__ int first_odd[DP]; /* the first key whose value is not finite there */
+    __shared__ uint32_t seat;
     __shared__ float joined[WK > 1 ? WK : 1][2][32];
 
     const AttnTokens &a = p.t;
@@ -288,6 +289,9 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     AttnItem it;
     if (!find_item<S::ROWS, KT * WK>(p, gridDim.x / a.kv_heads - 1 - item, lane, &it)) return;
 
+
+    for (int i = tid; i < DP; i += THREADS) first_odd[i] = INT32_MAX;
+    lds_barrier();
 
     /* the keys of this piece */
     const int last_token = min(it.n - 1, (it.tile * S::ROWS + S::ROWS - 1) / group);
@@ -365,7 +369,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             }
         }
     };
-    auto store = [&](bool masked) {
+    auto store = [&](int k0) {
+        const bool masked = k0 + KT - 1 > unmasked;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const int b = unit_block(u);
@@ -393,9 +398,22 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                                 top = max(top, max(m0 >= inf ? 0u : m0, m1 >= inf ? 0u : m1));
                             }
                         }
-                if (values) {
-                    const bool any = __any(odd);
-                    if (lane == 0) not_finite[wk][b] = any;
+                /* A value that is not finite must not reach the rows that do not
+                 * attend it, and 0 * inf is NaN: where some do not, zero takes its
+                 * place here, and the rows that do are marked at the end. */
+                if (values && masked && __any(odd)) {
+#pragma unroll
+                    for (int i = 0; i < SLOTS; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            constexpr bool wide = TYPE == QMV_KV_F32;
+                            const uint32_t w = raw[u][i][wide ? e >> 2 : 0][wide ? e & 3 : e >> 1];
+                            const uint32_t mask = wide ? inf : inf << 16 * (e & 1);
+                            if ((w & mask) == mask) {
+                                raw[u][i][wide ? e >> 2 : 0][wide ? e & 3 : e >> 1] = wide ? 0u : w & 0xffff0000u >> 16 * (e & 1);
+                                atomicMin(&first_odd[8 * piece + e], k0 + 16 * b + i * PER + sub);
+                            }
+                        }
                 }
                 if (TYPE != QMV_KV_F16) {
                     top = wave_max(top);
@@ -459,6 +477,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     auto compute = [&](int k0) {
 #pragma unroll
         for (int sb = 0; sb < KT / 32; ++sb) {
+            __builtin_amdgcn_sched_barrier(0);
             f16_t c = {0};
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
@@ -518,43 +537,12 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int step = 2 * sb + g;
-                if (masked && not_finite[wk][step]) {
-                    /* A value that is not finite must not reach the rows that do
-                     * not attend it, and 0 * inf is NaN: its place is zero in the
-                     * product, and a product of marks finds the rows that do. */
-                    h8_t seen;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        seen[i] = (_Float16)(first + 16 * g + 8 * (i >> 2) + (i & 3) <= pos ? 1.f : 0.f);
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        h8_t v = v_frag(0, step, db), mark;
-                        h8_t v2 = NL == 2 ? v_frag(1, step, db) : v;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const _Float16 x = v[i];
-                            const bool odd = (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00;
-                            mark[i] = (_Float16)(odd ? 1.f : 0.f);
-                            if (odd) v[i] = v2[i] = (_Float16)0.f;
-                        }
-                        f16_t hits = {0};
-                        hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(mark, seen, hits, 0, 0, 0);
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
-                        if (NL == 2) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, phi[g], o[db], 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (hits[i] > 0.f) o[db][i] = NAN;
-                    }
-                } else {
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        const h8_t v = v_frag(0, step, db);
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
-                        if (NL == 2)
-                            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(1, step, db), phi[g], o[db], 0, 0, 0);
-                    }
+                for (int db = 0; db < DB; ++db) {
+                    const h8_t v = v_frag(0, step, db);
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
+                    if (NL == 2) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(1, step, db), phi[g], o[db], 0, 0, 0);
                 }
             }
         }
@@ -567,7 +555,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     next = place(k0 + STEP);
     for (int at = begin; at < end; at += STEP, k0 += STEP) {
         if (WR > 1) lds_barrier(); /* the last tile has been read */
-        store(k0 + KT - 1 > unmasked);
+        store(k0);
         if (at + STEP < end) load(next);
         next = place(k0 + 2 * STEP);
         if (WR > 1) lds_barrier();
@@ -594,6 +582,9 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             for (int j = 0; j < 4; ++j) {
                 const int d = 32 * db + 8 * j + 4 * half;
                 f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (pos >= first_odd[d + i]) v[i] = NAN;
                 if (pieces == 1) {
                     v = none ? f4_t{0, 0, 0, 0} : v * kDown / l;
                     if (out != nullptr && d < dim) *(f4_t *)(out + d) = v;
@@ -637,6 +628,10 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
                 v += *(const f4_t *)((const float *)lds + w * 32 * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
             }
+            const int rr_row = it.tile * S::ROWS + rr, rr_pos = it.first + rr_row / group;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (rr_pos >= first_odd[4 * d4 + i]) v[i] = NAN;
             if (pieces == 1) {
                 float *out = out_of(rr);
                 v = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
@@ -654,11 +649,10 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     /* The last of a row tile's pieces joins them, in their order. */
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     lds_barrier();
-    uint32_t *const seat = &not_finite[0][0];
     unsigned *const counter = p.counters + (int64_t)it.tile_at * a.kv_heads + kvh;
-    if (tid == 0) *seat = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) seat = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     lds_barrier();
-    if (*seat != (uint32_t)pieces - 1u) return;
+    if (seat != (uint32_t)pieces - 1u) return;
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const float *first_part = part - (int64_t)it.split * a.kv_heads * S::PARTIAL;
     const int64_t apart = (int64_t)a.kv_heads * S::PARTIAL;
