@@ -56,7 +56,6 @@ __device__ __forceinline__ int64_t key_at(const AttnTokens &a, int s, int start,
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef float f16_t __attribute__((ext_vector_type(16)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
@@ -73,18 +72,44 @@ __device__ __forceinline__ void lds_barrier()
     asm volatile("" ::: "memory");
 }
 
-/* The larger of this lane's and lane ^ 32's. */
-__device__ __forceinline__ float max_halves(float x)
+/* The values of the lanes that share lane % RW (32 or 16), joined by f. */
+template <int RW, typename F> __device__ __forceinline__ float join_lanes(float x, F f)
 {
+    if (RW == 16) {
+        const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    }
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int RW> __device__ __forceinline__ float max_lanes(float x)
+{
+    return join_lanes<RW>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int RW> __device__ __forceinline__ float sum_lanes(float x)
+{
+    return join_lanes<RW>(x, [](float a, float b) { return a + b; });
 }
 
-__device__ __forceinline__ float sum_halves(float x)
-{
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
+/* Matrix products of RW columns, D (RW x RW) += A B: a lane holds 8 elements of
+ * the contraction of one row of A and of one column of B, lane % RW, those
+ * from 8 (lane / RW) on (of 16 with RW = 32, of 32 with RW = 16); and of D's
+ * column lane % RW the rows 4 (lane / RW) + 256 / RW j + i in register 4 j + i. */
+template <int RW> struct Product;
+template <> struct Product<32> {
+    typedef float acc_t __attribute__((ext_vector_type(16)));
+    static __device__ __forceinline__ acc_t run(h8_t a, h8_t b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Product<16> {
+    typedef float acc_t __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ acc_t run(h8_t a, h8_t b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
 
 /* The largest of the wave's unsigned values, in every lane. */
 __device__ __forceinline__ uint32_t wave_max(uint32_t v)
@@ -119,16 +144,17 @@ __device__ __forceinline__ f2_t load_shared(const float *p)
 
 /* ---- attention -----------------------------------------------------------------
  *
- * A workgroup takes a tile of 32 WR rows of one sequence and key head, a row
+ * A workgroup takes a tile of RW WR rows of one sequence and key head, a row
  * being a new token and one of the group's query heads, so every key and value
- * that it reads serves the whole group; and a range of keys. A wave holds 32
- * rows; WK waves take turns along the keys. Per 32 keys it computes
+ * that it reads serves the whole group; and a range of keys. A wave holds RW
+ * rows (32, or 16 where a sequence has no more); WK waves take turns along the
+ * keys. Per 32 keys it computes
  *   S^T = K Q^T   (matrix rows: keys; columns: rows of the tile)
  *   O^T += V^T P^T
- * with 32x32x16 products: a lane has one row's scores in its registers, and the
- * registers that S^T leaves are the operand that O^T's product takes, with no
- * exchange between lanes, if V's keys are read in the same order. The running
- * maximum and sum are a lane's own, its other half's apart.
+ * A lane has scores of one row in its registers, and the registers that S^T
+ * leaves are the operand that O^T's product takes, with no exchange between
+ * lanes, if V's keys are read in the same order. The running maximum is joined
+ * over the lanes of a row, the sum at the end.
  *
  * Numbers. Products are of f16 with fp32 sums. q (times scale and log2 e) and
  * the weights are two f16 limbs each, x = hi + lo, after a power of two has
@@ -253,9 +279,9 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     return false;
 }
 
-/* DP: head_dim padded to 64 or 128; WR waves along the rows, WK along the
- * keys. */
-template <int TYPE, int DP, int WR, int WK> struct AttnShape {
+/* DP: head_dim padded to 64 or 128; RW: rows of a wave; WR waves along the
+ * rows, WK along the keys. */
+template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int NL = TYPE == QMV_KV_F32 ? 2 : 1;   /* limbs of keys and values */
     static constexpr int KT = WR >= 4 ? 64 : 32;            /* keys a wave takes per tile */
     static constexpr int NB = KT / 16;                      /* blocks of 16 keys */
@@ -263,27 +289,30 @@ template <int TYPE, int DP, int WR, int WK> struct AttnShape {
     static constexpr int SLOTS = DP / 32;                   /* pieces of 8 elements a lane loads per block */
     static constexpr int MAT = KT * DP * 2;                 /* bytes of a limb of keys or of values */
     static constexpr int TILE = 2 * NL * MAT;
-    static constexpr int ROWS = 32 * WR;
-    static constexpr int JOIN = WK > 1 ? WK * (32 * DP * 4) : 0; /* the waves' O, where they meet */
+    static constexpr int ROWS = RW * WR;
+    static constexpr int JOIN = WK > 1 ? WK * (RW * DP * 4) : 0; /* the waves' O, where they meet */
     static constexpr int LDS = WK * TILE > JOIN ? WK * TILE : JOIN;
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
 };
 
-template <int TYPE, int DP, int WR, int WK>
+template <int TYPE, int DP, int RW, int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 {
-    using S = AttnShape<TYPE, DP, WR, WK>;
+    using S = AttnShape<TYPE, DP, RW, WR, WK>;
+    using P = Product<RW>;
+    using acc_t = typename P::acc_t;
     constexpr int KT = S::KT, NB = S::NB, UNITS = S::UNITS, SLOTS = S::SLOTS, MAT = S::MAT, NL = S::NL;
-    constexpr int THREADS = 64 * WR * WK, STEPS = DP / 16, DB = DP / 32;
+    constexpr int THREADS = 64 * WR * WK, WIDE = 512 / RW; /* of a product's contraction */
+    constexpr int STEPS = DP / WIDE, DB = DP / RW, REGS = RW * RW / 64, SCORES = RW / 2;
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
     __shared__ float scales[WK][2 * NB]; /* of the keys: factors; of the values: exponents */
     __shared__ int first_odd[DP]; /* the first key whose value is not finite there */
     __shared__ uint32_t seat;
-    __shared__ float joined[WK > 1 ? WK : 1][2][32];
+    __shared__ float joined[WK > 1 ? WK : 1][2][RW];
 
     const AttnTokens &a = p.t;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wave % WR, wk = wave / WR, half = lane >> 5, col = lane & 31;
+    const int wr = wave % WR, wk = wave / WR, part_of = lane / RW, col = lane % RW;
     const int group = a.heads / a.kv_heads, dim = a.dim;
     const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
     AttnItem it;
@@ -301,8 +330,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     const int begin = it.split * it.chunk, end = min((int64_t)keys, (int64_t)begin + it.chunk);
     const int unmasked = it.first + it.tile * S::ROWS / group; /* every row attends keys up to here */
 
-    /* this lane's row: q as two limbs, its 8 elements of each 16-wide step */
-    const int row = it.tile * S::ROWS + wr * 32 + col;
+    /* this lane's row: q as two limbs, 8 elements of each step */
+    const int row = it.tile * S::ROWS + wr * RW + col;
     const int token = row / group, head = kvh * group + row % group;
     const bool real = token < it.n;
     const int pos = real ? it.first + token : -1;
@@ -315,7 +344,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         uint32_t bits = 0;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) {
-            const int d = 16 * st + 8 * half;
+            const int d = WIDE * st + 8 * part_of;
             f4_t u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
             if (real && d < dim) {
                 u = *(const f4_t *)(q + d);
@@ -328,8 +357,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 if (m < 0x7f800000u) bits = max(bits, m);
             }
         }
-        const auto both = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
-        const int n = scale_of(max((uint32_t)both[0], (uint32_t)both[1]), 126);
+        const int n = scale_of(__float_as_uint(max_lanes<RW>(__uint_as_float(bits))), 126);
         q_back = power_of_two(-n);
 #pragma unroll
         for (int st = 0; st < STEPS; ++st) limbs_of(x[st], power_of_two(n), &qhi[st], &qlo[st]);
@@ -450,27 +478,34 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     };
 
     /* ---- a tile's products ---- */
-    f16_t o[DB];
+    acc_t o[DB];
 #pragma unroll
-    for (int i = 0; i < DB; ++i) o[i] = f16_t{0};
+    for (int i = 0; i < DB; ++i) o[i] = acc_t{0};
     float r = kNothing, l = 0.f;
+    /* Key 32 sb + score_key(i) of a tile is the one of score register i. */
+    auto score_key = [&](int i) { return (256 / RW) * (i >> 2) + 4 * part_of + (i & 3); };
     const int turn_k = DP == 128 ? (col & 3) << 2 | (col >> 2 & 3) : (col >> 1 & 1) << 2 | (col >> 2 & 3);
-    const int k_at = col * DP * 2 + ((half ^ turn_k) << 4);
+    const int k_at = col * DP * 2 + ((part_of ^ turn_k) << 4);
+    /* K of RW keys, one step of the contraction. */
+    auto k_frag = [&](int limb, int kb, int st) -> h8_t {
+        return *(const h8_t *)(tile + limb * MAT + kb * RW * DP * 2 + (k_at ^ st * (WIDE * 2)));
+    };
     const int kk = (lane & 15) >> 2; /* this lane's key of four in a transposing load */
     int v_at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int key = 8 * i + 4 * half + kk;
-        const int low = ((lane >> 4 & 1) << 1 | (lane >> 1 & 1)) ^ (2 * i + half);
-        v_at[i] = key * DP * 2 + ((DP == 128 ? kk << 2 : (kk >> 1) << 2) + low) * 16 + (lane & 1) * 8;
+        const int key = 256 / RW * i + 4 * part_of + kk;
+        const int turn = DP == 128 ? kk << 2 | (key >> 2 & 3) : (kk >> 1) << 2 | (key >> 2 & 3);
+        const int at = (RW == 32 ? (lane >> 4 & 1) << 1 : 0) | (lane >> 1 & 1); /* pieces within the product's rows */
+        v_at[i] = key * DP * 2 + ((at ^ turn) << 4) + (lane & 1) * 8;
     }
-    /* V^T of 16 keys and 32 elements: 8 keys of one element a lane, in the order
-     * in which the scores are in its registers. */
+    /* V^T of one step of keys and RW elements: 8 keys of one element a lane, in
+     * the order in which the scores are in its registers. */
     auto v_frag = [&](int limb, int step, int db) -> h8_t {
-        const unsigned char *base = tile + (NL + limb) * MAT + step * 16 * DP * 2;
+        const unsigned char *base = tile + (NL + limb) * MAT + step * WIDE * DP * 2;
         typedef QMV_LDS s4_t *ptr;
-        const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[0] ^ db << 6)));
-        const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[1] ^ db << 6)));
+        const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[0] ^ db * (RW * 2))));
+        const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(base + (v_at[1] ^ db * (RW * 2))));
         const h4_t hx = __builtin_bit_cast(h4_t, x), hy = __builtin_bit_cast(h4_t, y);
         return h8_t{hx[0], hx[1], hx[2], hx[3], hy[0], hy[1], hy[2], hy[3]};
     };
@@ -478,21 +513,26 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 #pragma unroll
         for (int sb = 0; sb < KT / 32; ++sb) {
             __builtin_amdgcn_sched_barrier(0);
-            f16_t c = {0};
+            float c[SCORES];
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-                const unsigned char *at = tile + 32 * sb * DP * 2 + (k_at ^ st << 5);
-                const h8_t hi = *(const h8_t *)at;
-                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[st], c, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[st], c, 0, 0, 0);
-                if (NL == 2) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8_t *)(at + MAT), qhi[st], c, 0, 0, 0);
+            for (int kb = 0; kb < 32 / RW; ++kb) {
+                acc_t x = {0};
+#pragma unroll
+                for (int st = 0; st < STEPS; ++st) {
+                    const h8_t hi = k_frag(0, 32 / RW * sb + kb, st);
+                    x = P::run(hi, qhi[st], x);
+                    x = P::run(hi, qlo[st], x);
+                    if (NL == 2) x = P::run(k_frag(1, 32 / RW * sb + kb, st), qhi[st], x);
+                }
+#pragma unroll
+                for (int i = 0; i < REGS; ++i) c[REGS * kb + i] = x[i];
             }
-            const int first = k0 + 32 * sb + 4 * half; /* key of register 8 g + i: first + 16 g + 8 (i / 4) + i % 4 */
-            const bool masked = k0 + 32 * sb + 31 > unmasked;
+            const int first = k0 + 32 * sb;
+            const bool masked = first + 31 > unmasked;
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (first + 8 * (i >> 2) + (i & 3) > pos) c[i] = -INFINITY;
+                for (int i = 0; i < SCORES; ++i)
+                    if (first + score_key(i) > pos) c[i] = -INFINITY;
             }
             float by[2], add[2], back[2];
             float top = -INFINITY;
@@ -507,12 +547,13 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                     add[g] = scales[wk][NB + 2 * sb + g];
                     back[g] = __builtin_ldexpf(1.f, -20 - (int)add[g]); /* may be a denormal */
                 }
-                float m = c[8 * g];
+                constexpr int EACH = SCORES / 2; /* scores of a block of 16 keys */
+                float m = c[EACH * g];
 #pragma unroll
-                for (int i = 1; i < 8; ++i) m = fmaxf(m, c[8 * g + i]);
+                for (int i = 1; i < EACH; ++i) m = fmaxf(m, c[EACH * g + i]);
                 top = fmaxf(top, fmaf(m, by[g], add[g]));
             }
-            top = max_halves(top);
+            top = max_lanes<RW>(top);
             if (__any(top > r + kSlack)) {
                 const float to = top > r + kSlack ? top : r;
                 const float fade = __builtin_amdgcn_exp2f(r - to);
@@ -521,28 +562,29 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[i] *= fade;
             }
-            h8_t phi[2], plo[2];
+            constexpr int VS = 32 / WIDE; /* steps of 8 scores a lane */
+            h8_t phi[VS], plo[VS];
+            float w[SCORES];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const float shift = add[g] - r + kShift;
-                float w[8], sum = 0.f;
+                float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(fmaf(c[8 * g + i], by[g], shift));
+                for (int i = SCORES / 2 * g; i < SCORES / 2 * (g + 1); ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(fmaf(c[i], by[g], shift));
                     sum += w[i];
                 }
-                limbs_of(w, 1.f, &phi[g], &plo[g]);
                 l = TYPE == QMV_KV_F16 ? l + sum : fmaf(sum, back[g], l);
             }
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int step = 2 * sb + g;
+            for (int g = 0; g < VS; ++g) {
+                limbs_of(w + 8 * g, 1.f, &phi[g], &plo[g]);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
-                    const h8_t v = v_frag(0, step, db);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, phi[g], o[db], 0, 0, 0);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, plo[g], o[db], 0, 0, 0);
-                    if (NL == 2) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(1, step, db), phi[g], o[db], 0, 0, 0);
+                    const h8_t v = v_frag(0, VS * sb + g, db);
+                    o[db] = P::run(v, phi[g], o[db]);
+                    o[db] = P::run(v, plo[g], o[db]);
+                    if (NL == 2) o[db] = P::run(v_frag(1, VS * sb + g, db), phi[g], o[db]);
                 }
             }
         }
@@ -563,7 +605,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         if (k0 < end) compute(k0);
         if (WR == 1) asm volatile("" ::: "memory");
     }
-    l = sum_halves(l);
+    l = sum_lanes<RW>(l);
     constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
     const int64_t slot = (int64_t)(gridDim.x / a.kv_heads - 1 - item) * a.kv_heads + kvh; /* of split 0: less split * kv_heads */
     float *const part = p.partials + slot * S::PARTIAL;
@@ -573,14 +615,14 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     };
 
     if (WK == 1) {
-        /* register 4 j + i of o[db]: element 32 db + 8 j + 4 half + i of this lane's row */
-        float *out = out_of(wr * 32 + col);
+        /* register 4 j + i of o[db]: element RW db + 8 j + 4 part_of + i of this lane's row */
+        float *out = out_of(wr * RW + col);
         const bool none = l == 0.f;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d = 32 * db + 8 * j + 4 * half;
+            for (int j = 0; j < REGS / 4; ++j) {
+                const int d = RW * db + 8 * j + 4 * part_of;
                 f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -588,16 +630,16 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 if (pieces == 1) {
                     v = none ? f4_t{0, 0, 0, 0} : v * kDown / l;
                     if (out != nullptr && d < dim) *(f4_t *)(out + d) = v;
-                } else {
-                    float *to = part + (wr * 32 + col) * DP + d;
+                } else if (real) {
+                    float *to = part + (wr * RW + col) * DP + d;
                     store_shared(to, v[0], v[1]);
                     store_shared(to + 2, v[2], v[3]);
                 }
             }
-        if (pieces > 1 && half == 0) store_shared(part + S::ROWS * DP + 2 * (wr * 32 + col), r, l);
+        if (pieces > 1 && part_of == 0 && real) store_shared(part + S::ROWS * DP + 2 * (wr * RW + col), r, l);
     } else {
         /* the waves' results meet in LDS */
-        if (half == 0) {
+        if (part_of == 0) {
             joined[wk][0][col] = r;
             joined[wk][1][col] = l;
         }
@@ -605,19 +647,19 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         float top = joined[0][0][col];
 #pragma unroll
         for (int w = 1; w < WK; ++w) top = fmaxf(top, joined[w][0][col]);
-        float *mine = (float *)lds + wk * 32 * DP;
+        float *mine = (float *)lds + wk * RW * DP;
         const float fade = __builtin_amdgcn_exp2f(r - top);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int d4 = 8 * db + 2 * j + half;
+            for (int j = 0; j < REGS / 4; ++j) {
+                const int d4 = RW / 4 * db + 2 * j + part_of;
                 const f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
                 *(f4_t *)(mine + col * DP + ((d4 ^ (col & 7)) << 2)) = v * fade;
             }
         lds_barrier();
 #pragma unroll
-        for (int e = tid; e < 32 * DP / 4; e += THREADS) {
+        for (int e = tid; e < RW * DP / 4; e += THREADS) {
             const int rr = e / (DP / 4), d4 = e % (DP / 4);
             float all = joined[0][0][rr], sum = 0.f;
 #pragma unroll
@@ -626,16 +668,17 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 #pragma unroll
             for (int w = 0; w < WK; ++w) {
                 sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
-                v += *(const f4_t *)((const float *)lds + w * 32 * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
+                v += *(const f4_t *)((const float *)lds + w * RW * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
             }
             const int rr_row = it.tile * S::ROWS + rr, rr_pos = it.first + rr_row / group;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (rr_pos >= first_odd[4 * d4 + i]) v[i] = NAN;
+            float *out = out_of(rr);
+            if (out == nullptr) continue;
             if (pieces == 1) {
-                float *out = out_of(rr);
                 v = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
-                if (out != nullptr && 4 * d4 < dim) *(f4_t *)(out + 4 * d4) = v;
+                if (4 * d4 < dim) *(f4_t *)(out + 4 * d4) = v;
             } else {
                 float *to = part + rr * DP + 4 * d4;
                 store_shared(to, v[0], v[1]);
@@ -661,29 +704,50 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         float *out = out_of(rr);
         if (out == nullptr || 4 * d4 >= dim) continue;
         const float *state = first_part + S::ROWS * DP + 2 * rr, *val = first_part + rr * DP + 4 * d4;
+        constexpr int AT_ONCE = 16; /* pieces whose loads are in flight together */
         float all = kNothing, sum = 0.f;
-        for (int i = 0; i < pieces; ++i) all = fmaxf(all, load_shared(state + i * apart)[0]);
         f4_t v = {0, 0, 0, 0};
-        for (int i = 0; i < pieces; ++i) {
-            const f2_t st = load_shared(state + i * apart);
-            const f2_t x = load_shared(val + i * apart), y = load_shared(val + i * apart + 2);
-            const float fade = __builtin_amdgcn_exp2f(st[0] - all);
-            sum = fmaf(st[1], fade, sum);
-            v += f4_t{x[0], x[1], y[0], y[1]} * fade;
+        for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
+            f2_t st[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int64_t from = min(i0 + i, pieces - 1) * apart;
+                st[i] = load_shared(state + from);
+                x[i] = load_shared(val + from);
+                y[i] = load_shared(val + from + 2);
+            }
+            float top = all;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, st[i][0]);
+            const float fade = __builtin_amdgcn_exp2f(all - top);
+            all = top;
+            sum *= fade;
+            v *= fade;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const float f = i0 + i < pieces ? __builtin_amdgcn_exp2f(st[i][0] - all) : 0.f;
+                if (i0 + i < pieces) {
+                    sum = fmaf(st[i][1], f, sum);
+                    v += f4_t{x[i][0], x[i][1], y[i][0], y[i][1]} * f;
+                }
+            }
         }
         *(f4_t *)(out + 4 * d4) = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
     }
 }
 
+#ifndef QMV_ATTN_TARGET
+#define QMV_ATTN_TARGET 512
+#endif
 AttnPlan plan_attention(const AttnTokens &t)
 {
     AttnPlan plan = {};
     const int group = t.heads / t.kv_heads;
     const int64_t rows = (int64_t)t.tokens * group, each = rows / t.count;
-    plan.rows = each <= 48 ? 32 : each <= 1024 ? 128 : 256;
+    plan.rows = each <= 16 ? 16 : each <= 48 ? 32 : each <= 1024 ? 128 : 256;
     const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
     plan.tiles = (int)tiles;
-    plan.target = tiles * t.kv_heads < 2048 ? 512 : 0;
+    plan.target = tiles * t.kv_heads < 2048 ? QMV_ATTN_TARGET : 0;
     const int64_t items = tiles + (plan.target ? plan.target / t.kv_heads + 1 : 0);
     plan.grid = items * t.kv_heads;
     if (plan.target) {
@@ -697,9 +761,10 @@ AttnPlan plan_attention(const AttnTokens &t)
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     const dim3 grid((unsigned)plan.grid);
-    if (plan.rows == 32) attention_kernel<TYPE, DP, 1, 4><<<grid, 256, 0, s>>>(p);
-    else if (plan.rows == 128) attention_kernel<TYPE, DP, 4, 1><<<grid, 256, 0, s>>>(p);
-    else attention_kernel<TYPE, DP, 8, 1><<<grid, 512, 0, s>>>(p);
+    if (plan.rows == 16) attention_kernel<TYPE, DP, 16, 1, 4><<<grid, 256, 0, s>>>(p);
+    else if (plan.rows == 32) attention_kernel<TYPE, DP, 32, 1, 4><<<grid, 256, 0, s>>>(p);
+    else if (plan.rows == 128) attention_kernel<TYPE, DP, 32, 4, 1><<<grid, 256, 0, s>>>(p);
+    else attention_kernel<TYPE, DP, 32, 8, 1><<<grid, 512, 0, s>>>(p);
 }
 
 template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
