@@ -131,15 +131,24 @@ __device__ __forceinline__ int64_t shfl64(int64_t v, int lane)
     return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 
-/* Agent-scope stores and loads of what workgroups pass to each other. */
-__device__ __forceinline__ void store_shared(float *p, float a, float b)
+/* Sums over the lanes up to each: of row_shr 1, 2, 4, 8 within rows of 16, then
+ * of the rows before. */
+template <typename T> __device__ __forceinline__ T scan_lanes(T v)
 {
-    const f2_t v = {a, b};
-    __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#define QMV_STEP(CTRL, ROWS) \
+    v += __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    QMV_STEP(0x111, 0xf)
+    QMV_STEP(0x112, 0xf)
+    QMV_STEP(0x114, 0xf)
+    QMV_STEP(0x118, 0xf)
+    QMV_STEP(0x142, 0xa)
+    QMV_STEP(0x143, 0xc)
+#undef QMV_STEP
+    return v;
 }
-__device__ __forceinline__ f2_t load_shared(const float *p)
+template <typename T> __device__ __forceinline__ T lane_of(T v, int lane)
 {
-    return __builtin_bit_cast(f2_t, __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
 /* ---- attention -----------------------------------------------------------------
@@ -205,15 +214,24 @@ struct AttnItem {
     int split, chunk;     /* keys [split * chunk, ...) */
 };
 
+/* What the pieces' join has to know of a row tile whose keys are cut. */
+struct AttnJoin {
+    int start, n, tile; /* as in AttnItem */
+    int pieces, item;   /* how many, and which was the first; 0: not cut */
+};
+
 /* The `item`-th piece of a key head's work, by one wave: the sequences' row
- * tiles, each cut into pieces of `chunk` keys, one after the other. chunk is
- * chosen here from all lengths, so every workgroup has the same. */
+ * tiles, the later ones (which attend more) first, each cut into pieces of
+ * `chunk` keys. chunk is chosen here from all lengths, so that every workgroup
+ * has the same; the sums are of floats, whose rounding the one piece beyond
+ * plan_attention's count allows for. *tiles_all: row tiles in all, or 0 where
+ * the starts fall so that there would be more rows than the call's. */
 template <int BM, int STEP>
-__device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lane, AttnItem *out)
+__device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lane, AttnItem *out, int *tiles_all)
 {
     const AttnTokens &a = p.t;
     const int group = a.heads / a.kv_heads;
-    const int64_t room = a.page_size ? (int64_t)a.table_stride * a.page_size : INT32_MAX;
+    const int room = a.page_size ? a.table_stride * a.page_size : INT32_MAX; /* at most 2^30, or no limit */
     int start = 0, n = 0, len = 0, first = 0, tiles = 0;
     auto read = [&](int s) {
         start = n = len = first = tiles = 0;
@@ -222,61 +240,53 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
         n = max(min(a.starts[s + 1], a.tokens) - start, 0);
         len = a.lengths ? max(a.lengths[s], 0) : n;
         first = len - n;
-        if (len > room) len = (int)room + 1; /* one key past the table: its rows are NaN */
-        tiles = (int)(((int64_t)n * group + BM - 1) / BM);
+        if (len > room) len = room + 1; /* one key past the table: its rows are NaN */
+        tiles = (n * group + BM - 1) / BM;
     };
-    int64_t work = 0, rows = 0;
+    float work = 0.f, rows = 0.f;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         read(s0 + lane);
-        work += (int64_t)tiles * len;
-        rows += n;
+        work += (float)tiles * (float)len;
+        rows += (float)n;
     }
-#pragma unroll
-    for (int i = 32; i; i >>= 1) {
-        work += shfl64(work, lane ^ i);
-        rows += shfl64(rows, lane ^ i);
-    }
-    if (rows > a.tokens) return false; /* starts that fall */
-    int64_t chunk = INT32_MAX / STEP * STEP;
+    work = lane_of(scan_lanes(work), 63);
+    rows = lane_of(scan_lanes(rows), 63);
+    *tiles_all = 0;
+    if (rows > (float)a.tokens) return false;
+    int chunk = INT32_MAX / STEP * STEP;
     if (p.target) {
-        const int64_t pieces = max(p.target / a.kv_heads, 1);
-        chunk = max((work + pieces - 1) / pieces, (int64_t)2 * STEP);
-        chunk = (chunk + STEP - 1) / STEP * STEP;
+        const float each = work / (float)max(p.target / a.kv_heads, 1);
+        chunk = each < 1e9f ? max(((int)each + STEP) / STEP * STEP, 2 * STEP) : chunk;
     }
     int before = 0, tiles_before = 0;
+    bool found = false;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         if (a.count > 64) read(s0 + lane);
-        const int splits = max((int)((len + chunk - 1) / chunk), 1);
+        const int splits = max((int)(((uint32_t)len + (uint32_t)chunk - 1) / (uint32_t)chunk), 1);
         const int items = tiles * splits;
-        int sum = items, tsum = tiles;
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) {
-            const int u = __shfl_up(sum, i), v = __shfl_up(tsum, i);
-            if (lane >= i) {
-                sum += u;
-                tsum += v;
-            }
-        }
+        const int sum = scan_lanes(items), tsum = scan_lanes(tiles);
         const uint64_t hit = __ballot(before + sum > item);
-        if (hit) {
+        if (hit && !found) {
             const int at = __builtin_ctzll(hit);
-            const int mine = item - before - (__shfl(sum, at) - __shfl(items, at));
-            const int sp = __shfl(splits, at);
+            const int mine = item - before - (lane_of(sum, at) - lane_of(items, at));
+            const int sp = lane_of(splits, at), nth = mine / sp;
             out->s = s0 + at;
-            out->start = __shfl(start, at);
-            out->n = __shfl(n, at);
-            out->len = __shfl(len, at);
-            out->first = __shfl(first, at);
-            out->chunk = (int)chunk;
-            out->tile = mine / sp;
-            out->split = mine - out->tile * sp;
-            out->tile_at = tiles_before + __shfl(tsum, at) - __shfl(tiles, at) + out->tile;
-            return true;
+            out->start = lane_of(start, at);
+            out->n = lane_of(n, at);
+            out->len = lane_of(len, at);
+            out->first = lane_of(first, at);
+            out->chunk = chunk;
+            out->split = mine - nth * sp;
+            out->tile = lane_of(tiles, at) - 1 - nth;
+            out->tile_at = tiles_before + lane_of(tsum, at) - lane_of(tiles, at) + out->tile;
+            found = true;
         }
-        before += __shfl(sum, 63);
-        tiles_before += __shfl(tsum, 63);
+        before += lane_of(sum, 63);
+        tiles_before += lane_of(tsum, 63);
+        if (found && item > 0) break; /* the first workgroup counts all tiles */
     }
-    return false;
+    *tiles_all = tiles_before;
+    return found;
 }
 
 /* DP: head_dim padded to 64 or 128; RW: rows of a wave; WR waves along the
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
     __shared__ float scales[WK][2 * NB]; /* of the keys: factors; of the values: exponents */
     __shared__ int first_odd[DP]; /* the first key whose value is not finite there */
-    __shared__ uint32_t seat;
+    __shared__ int any_odd;
     __shared__ float joined[WK > 1 ? WK : 1][2][RW];
 
     const AttnTokens &a = p.t;
@@ -316,10 +326,14 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     const int group = a.heads / a.kv_heads, dim = a.dim;
     const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
     AttnItem it;
-    if (!find_item<S::ROWS, KT * WK>(p, gridDim.x / a.kv_heads - 1 - item, lane, &it)) return;
+    int tiles_all;
+    const bool found = find_item<S::ROWS, KT * WK>(p, item, lane, &it, &tiles_all);
+    if (blockIdx.x == 0 && p.target && tid == 0) p.joins[0].n = tiles_all;
+    if (!found) return;
 
 
     for (int i = tid; i < DP; i += THREADS) first_odd[i] = INT32_MAX;
+    if (tid == 0) any_odd = 0;
     lds_barrier();
 
     /* the keys of this piece */
@@ -327,42 +341,16 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     const int keys = max(min(it.first + last_token + 1, it.len), 0);
     const int pieces = max((int)(((int64_t)keys + it.chunk - 1) / it.chunk), 1);
     if (it.split >= pieces) return;
+    if (p.target && kvh == 0 && it.split == 0 && tid == 0)
+        p.joins[1 + it.tile_at] = AttnJoin{it.start, it.n, it.tile, pieces > 1 ? pieces : 0, item};
     const int begin = it.split * it.chunk, end = min((int64_t)keys, (int64_t)begin + it.chunk);
     const int unmasked = it.first + it.tile * S::ROWS / group; /* every row attends keys up to here */
 
-    /* this lane's row: q as two limbs, 8 elements of each step */
+    /* this lane's row */
     const int row = it.tile * S::ROWS + wr * RW + col;
     const int token = row / group, head = kvh * group + row % group;
     const bool real = token < it.n;
     const int pos = real ? it.first + token : -1;
-    h8_t qhi[STEPS], qlo[STEPS];
-    float q_back;
-    {
-        const float *q = p.q + (int64_t)(it.start + token) * p.q_stride + (int64_t)head * dim;
-        const float by = p.scale * kLog2e;
-        float x[STEPS][8];
-        uint32_t bits = 0;
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            const int d = WIDE * st + 8 * part_of;
-            f4_t u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-            if (real && d < dim) {
-                u = *(const f4_t *)(q + d);
-                v = *(const f4_t *)(q + d + 4);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[st][i] = (i < 4 ? u[i & 3] : v[i & 3]) * by;
-                const uint32_t m = __float_as_uint(x[st][i]) & 0x7fffffffu;
-                if (m < 0x7f800000u) bits = max(bits, m);
-            }
-        }
-        const int n = scale_of(__float_as_uint(max_lanes<RW>(__uint_as_float(bits))), 126);
-        q_back = power_of_two(-n);
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) limbs_of(x[st], power_of_two(n), &qhi[st], &qlo[st]);
-    }
-
     /* ---- tiles: loads into registers, then as f16 limbs into LDS ---- */
     unsigned char *const tile = lds + wk * S::TILE;
     constexpr int PIECES = DP / 8, PER = 64 / PIECES; /* of a key; keys per slot */
@@ -430,6 +418,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                  * attend it, and 0 * inf is NaN: where some do not, zero takes its
                  * place here, and the rows that do are marked at the end. */
                 if (values && masked && __any(odd)) {
+                    if (lane == 0) any_odd = 1;
 #pragma unroll
                     for (int i = 0; i < SLOTS; ++i)
 #pragma unroll
@@ -476,6 +465,41 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             }
         }
     };
+
+    constexpr int STEP = KT * WK;
+    int k0 = begin + wk * KT;
+    int64_t next = place(k0);
+    if (begin < end) load(next);
+    next = place(k0 + STEP);
+
+    /* q as two limbs, 8 elements of each step */
+    h8_t qhi[STEPS], qlo[STEPS];
+    float q_back;
+    {
+        const float *q = p.q + (int64_t)(it.start + token) * p.q_stride + (int64_t)head * dim;
+        const float by = p.scale * kLog2e;
+        float x[STEPS][8];
+        uint32_t bits = 0;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            const int d = WIDE * st + 8 * part_of;
+            f4_t u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+            if (real && d < dim) {
+                u = *(const f4_t *)(q + d);
+                v = *(const f4_t *)(q + d + 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[st][i] = (i < 4 ? u[i & 3] : v[i & 3]) * by;
+                const uint32_t m = __float_as_uint(x[st][i]) & 0x7fffffffu;
+                if (m < 0x7f800000u) bits = max(bits, m);
+            }
+        }
+        const int n = scale_of(__float_as_uint(max_lanes<RW>(__uint_as_float(bits))), 126);
+        q_back = power_of_two(-n);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) limbs_of(x[st], power_of_two(n), &qhi[st], &qlo[st]);
+    }
 
     /* ---- a tile's products ---- */
     acc_t o[DB];
@@ -590,11 +614,6 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         }
     };
 
-    constexpr int STEP = KT * WK;
-    int k0 = begin + wk * KT;
-    int64_t next = place(k0);
-    if (begin < end) load(next);
-    next = place(k0 + STEP);
     for (int at = begin; at < end; at += STEP, k0 += STEP) {
         if (WR > 1) lds_barrier(); /* the last tile has been read */
         store(k0);
@@ -607,36 +626,35 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     }
     l = sum_lanes<RW>(l);
     constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
-    const int64_t slot = (int64_t)(gridDim.x / a.kv_heads - 1 - item) * a.kv_heads + kvh; /* of split 0: less split * kv_heads */
-    float *const part = p.partials + slot * S::PARTIAL;
-    auto out_of = [&](int row_in_tile) -> float * {
-        const int rr = it.tile * S::ROWS + row_in_tile, tk = rr / group;
-        return tk < it.n ? p.out + (int64_t)(it.start + tk) * p.out_stride + (int64_t)(kvh * group + rr % group) * dim : nullptr;
-    };
+    float *const part = p.partials + (int64_t)blockIdx.x * S::PARTIAL;
 
     if (WK == 1) {
         /* register 4 j + i of o[db]: element RW db + 8 j + 4 part_of + i of this lane's row */
-        float *out = out_of(wr * RW + col);
-        const bool none = l == 0.f;
+        const int row_in_tile = wr * RW + col;
+        float *to = pieces > 1 ? part + row_in_tile * DP
+                               : p.out + (int64_t)(it.start + token) * p.out_stride + (int64_t)head * dim;
+        const float by = pieces > 1 ? 1.f : l == 0.f ? 0.f : kDown / l;
+        const int width = pieces > 1 ? DP : dim;
+        if (any_odd) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < REGS; ++i)
+                    if (pos >= first_odd[RW * db + 8 * (i >> 2) + 4 * part_of + (i & 3)]) o[db][i] = NAN;
+        }
+        if (!real) return;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int j = 0; j < REGS / 4; ++j) {
                 const int d = RW * db + 8 * j + 4 * part_of;
-                f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (pos >= first_odd[d + i]) v[i] = NAN;
-                if (pieces == 1) {
-                    v = none ? f4_t{0, 0, 0, 0} : v * kDown / l;
-                    if (out != nullptr && d < dim) *(f4_t *)(out + d) = v;
-                } else if (real) {
-                    float *to = part + (wr * RW + col) * DP + d;
-                    store_shared(to, v[0], v[1]);
-                    store_shared(to + 2, v[2], v[3]);
-                }
+                const f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
+                if (d < width) *(f4_t *)(to + d) = v * by;
             }
-        if (pieces > 1 && part_of == 0 && real) store_shared(part + S::ROWS * DP + 2 * (wr * RW + col), r, l);
+        if (pieces > 1 && part_of == 0) {
+            const f2_t v = {r, l};
+            *(f2_t *)(part + S::ROWS * DP + 2 * row_in_tile) = v;
+        }
     } else {
         /* the waves' results meet in LDS */
         if (part_of == 0) {
@@ -658,8 +676,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 *(f4_t *)(mine + col * DP + ((d4 ^ (col & 7)) << 2)) = v * fade;
             }
         lds_barrier();
-#pragma unroll
-        for (int e = tid; e < RW * DP / 4; e += THREADS) {
+        const int rows = min(it.n * group - it.tile * S::ROWS, S::ROWS);
+        for (int e = tid; e < rows * (DP / 4); e += THREADS) {
             const int rr = e / (DP / 4), d4 = e % (DP / 4);
             float all = joined[0][0][rr], sum = 0.f;
 #pragma unroll
@@ -670,51 +688,63 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
                 v += *(const f4_t *)((const float *)lds + w * RW * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
             }
-            const int rr_row = it.tile * S::ROWS + rr, rr_pos = it.first + rr_row / group;
+            const int tile_row = it.tile * S::ROWS + rr, tk = tile_row / group;
+            if (any_odd) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (rr_pos >= first_odd[4 * d4 + i]) v[i] = NAN;
-            float *out = out_of(rr);
-            if (out == nullptr) continue;
+                for (int i = 0; i < 4; ++i)
+                    if (it.first + tk >= first_odd[4 * d4 + i]) v[i] = NAN;
+            }
             if (pieces == 1) {
-                v = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
+                float *out = p.out + (int64_t)(it.start + tk) * p.out_stride + (int64_t)(kvh * group + tile_row - tk * group) * dim;
+                v *= sum == 0.f ? 0.f : kDown / sum;
                 if (4 * d4 < dim) *(f4_t *)(out + 4 * d4) = v;
             } else {
-                float *to = part + rr * DP + 4 * d4;
-                store_shared(to, v[0], v[1]);
-                store_shared(to + 2, v[2], v[3]);
-                if (d4 == 0) store_shared(part + S::ROWS * DP + 2 * rr, all, sum);
+                *(f4_t *)(part + rr * DP + 4 * d4) = v;
+                if (d4 == 0) {
+                    const f2_t st = {all, sum};
+                    *(f2_t *)(part + S::ROWS * DP + 2 * rr) = st;
+                }
             }
         }
     }
-    if (pieces == 1) return;
+}
 
-    /* The last of a row tile's pieces joins them, in their order. */
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
-    unsigned *const counter = p.counters + (int64_t)it.tile_at * a.kv_heads + kvh;
-    if (tid == 0) seat = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    lds_barrier();
-    if (seat != (uint32_t)pieces - 1u) return;
-    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float *first_part = part - (int64_t)it.split * a.kv_heads * S::PARTIAL;
-    const int64_t apart = (int64_t)a.kv_heads * S::PARTIAL;
-    for (int e = tid; e < S::ROWS * DP / 4; e += THREADS) {
-        const int rr = e / (DP / 4), d4 = e % (DP / 4);
-        float *out = out_of(rr);
-        if (out == nullptr || 4 * d4 >= dim) continue;
-        const float *state = first_part + S::ROWS * DP + 2 * rr, *val = first_part + rr * DP + 4 * d4;
-        constexpr int AT_ONCE = 16; /* pieces whose loads are in flight together */
-        float all = kNothing, sum = 0.f;
-        f4_t v = {0, 0, 0, 0};
-        for (int i0 = 0; i0 < pieces; i0 += AT_ONCE) {
-            f2_t st[AT_ONCE], x[AT_ONCE], y[AT_ONCE];
+/* Joins the pieces of rows whose keys were cut, in their order within each of
+ * GROUPS groups of threads and then in the groups' order. A second kernel:
+ * joined by the last workgroup of a tile, the 128 pieces of one row tile at
+ * 32749 keys took 17 us of one compute unit. */
+template <int DP, int ROWS, int GROUPS>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float down)
+{
+    constexpr int D4 = DP / 4, EACH = 256 / (D4 * GROUPS); /* rows of a workgroup */
+    constexpr int AT_ONCE = 8;
+    constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
+    __shared__ f4_t sums[GROUPS > 1 ? GROUPS : 1][EACH][D4];
+    __shared__ f2_t states[GROUPS > 1 ? GROUPS : 1][EACH];
+    const AttnTokens &a = p.t;
+    const int slices = ROWS / EACH, group = a.heads / a.kv_heads;
+    const int slice = blockIdx.x % slices, rest = blockIdx.x / slices, kvh = rest % a.kv_heads, tile_at = rest / a.kv_heads;
+    if (tile_at >= p.joins[0].n) return;
+    const AttnJoin j = p.joins[1 + tile_at];
+    if (j.pieces == 0) return;
+    const int d4 = threadIdx.x % D4, set = threadIdx.x / D4 % GROUPS, rr = slice * EACH + threadIdx.x / (D4 * GROUPS);
+    const int row = j.tile * ROWS + rr, token = row / group;
+    if (j.tile * ROWS + slice * EACH >= j.n * group) return; /* no row of this workgroup */
+    const bool real = token < j.n;
+    const float *from = p.partials + ((int64_t)j.item * a.kv_heads + kvh) * PARTIAL;
+    const int64_t apart = (int64_t)a.kv_heads * PARTIAL;
+    const int mine = (j.pieces + GROUPS - 1) / GROUPS, i_end = min((set + 1) * mine, j.pieces);
+    float all = kNothing, sum = 0.f;
+    f4_t v = {0, 0, 0, 0};
+    if (real) {
+        for (int i0 = set * mine; i0 < i_end; i0 += AT_ONCE) {
+            f2_t st[AT_ONCE];
+            f4_t x[AT_ONCE];
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
-                const int64_t from = min(i0 + i, pieces - 1) * apart;
-                st[i] = load_shared(state + from);
-                x[i] = load_shared(val + from);
-                y[i] = load_shared(val + from + 2);
+                const float *at = from + min(i0 + i, i_end - 1) * apart;
+                st[i] = *(const f2_t *)(at + ROWS * DP + 2 * rr);
+                x[i] = *(const f4_t *)(at + rr * DP + 4 * d4);
             }
             float top = all;
 #pragma unroll
@@ -724,15 +754,35 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             sum *= fade;
             v *= fade;
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) {
-                const float f = i0 + i < pieces ? __builtin_amdgcn_exp2f(st[i][0] - all) : 0.f;
-                if (i0 + i < pieces) {
+            for (int i = 0; i < AT_ONCE; ++i)
+                if (i0 + i < i_end) {
+                    const float f = __builtin_amdgcn_exp2f(st[i][0] - all);
                     sum = fmaf(st[i][1], f, sum);
-                    v += f4_t{x[i][0], x[i][1], y[i][0], y[i][1]} * f;
+                    v += x[i] * f;
                 }
-            }
         }
-        *(f4_t *)(out + 4 * d4) = sum == 0.f ? f4_t{0, 0, 0, 0} : v * kDown / sum;
+    }
+    if (GROUPS > 1) {
+        const int e = threadIdx.x / (D4 * GROUPS);
+        sums[set][e][d4] = v;
+        if (d4 == 0) states[set][e] = f2_t{all, sum};
+        __syncthreads();
+        if (set > 0) return;
+        float top = all;
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, states[i][e][0]);
+        v = f4_t{0, 0, 0, 0};
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float f = __builtin_amdgcn_exp2f(states[i][e][0] - top);
+            sum = fmaf(states[i][e][1], f, sum);
+            v += sums[i][e][d4] * f;
+        }
+    }
+    if (real && 4 * d4 < a.dim) {
+        float *out = p.out + (int64_t)(j.start + token) * p.out_stride + (int64_t)(kvh * group + row - token * group) * a.dim;
+        *(f4_t *)(out + 4 * d4) = v * (sum == 0.f ? 0.f : down / sum);
     }
 }
 
@@ -752,19 +802,27 @@ AttnPlan plan_attention(const AttnTokens &t)
     plan.grid = items * t.kv_heads;
     if (plan.target) {
         const int dp = t.dim <= 64 ? 64 : 128;
+        plan.joins = (1 + (size_t)tiles) * sizeof(AttnJoin);
         plan.partials = (size_t)plan.grid * (plan.rows * (dp + 2));
-        plan.counters = (size_t)(tiles * t.kv_heads);
     }
     return plan;
 }
 
+template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+{
+    attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
+    if (plan.target == 0) return;
+    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
+    const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * (ROWS / EACH));
+    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
+}
+
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
-    const dim3 grid((unsigned)plan.grid);
-    if (plan.rows == 16) attention_kernel<TYPE, DP, 16, 1, 4><<<grid, 256, 0, s>>>(p);
-    else if (plan.rows == 32) attention_kernel<TYPE, DP, 32, 1, 4><<<grid, 256, 0, s>>>(p);
-    else if (plan.rows == 128) attention_kernel<TYPE, DP, 32, 4, 1><<<grid, 256, 0, s>>>(p);
-    else attention_kernel<TYPE, DP, 32, 8, 1><<<grid, 512, 0, s>>>(p);
+    if (plan.rows == 16) launch_shape<TYPE, DP, 16, 1, 4>(p, plan, s);
+    else if (plan.rows == 32) launch_shape<TYPE, DP, 32, 1, 4>(p, plan, s);
+    else if (plan.rows == 128) launch_shape<TYPE, DP, 32, 4, 1>(p, plan, s);
+    else launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
 }
 
 template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)

@@ -175,13 +175,12 @@ qmv::AttnTokens attn_tokens(const QmvSequences &q, int tokens, int heads, int kv
     return t;
 }
 
-/* What a stream's calls of few rows pass between workgroups. Buffers only grow,
- * and one that is replaced is kept: a graph captured earlier on the stream may
- * still use it (and every launch leaves its counters at zero). */
+/* What the pieces of a stream's calls leave for their join. The buffer only
+ * grows, and one that is replaced is kept: a graph captured earlier on the
+ * stream may still use it. */
 struct Workspace {
-    float *partials = nullptr;
-    unsigned *counters = nullptr;
-    size_t partial_cap = 0, counter_cap = 0;
+    unsigned char *data = nullptr;
+    size_t cap = 0;
     std::vector<void *> retired;
     std::mutex mu;
 };
@@ -197,34 +196,21 @@ Workspace &workspace_for(int device, hipStream_t stream)
     return *slot;
 }
 
-/* The workspace grown to a plan's need, its mutex held. New counters are cleared
- * on the stream by a kernel. */
-int workspace_reserve(Workspace &ws, hipStream_t stream, size_t partials, size_t counters)
+/* The workspace grown to `bytes`, its mutex held. */
+int workspace_reserve(Workspace &ws, hipStream_t stream, size_t bytes)
 {
-    if (partials <= ws.partial_cap && counters <= ws.counter_cap) return 1;
+    if (bytes <= ws.cap) return 1;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
         set_error("workspace must grow during stream capture; run the call once before capturing");
         return 0;
     }
-    if (partials > ws.partial_cap) {
-        const size_t n = partials + partials / 4;
-        void *buf = nullptr;
-        HIP_TRY(qmv::shim_malloc(&buf, n * sizeof(float)));
-        if (ws.partials) ws.retired.push_back(ws.partials);
-        ws.partials = (float *)buf;
-        ws.partial_cap = n;
-    }
-    if (counters > ws.counter_cap) {
-        const size_t n = counters + counters / 4 + 1024;
-        void *buf = nullptr;
-        HIP_TRY(qmv::shim_malloc(&buf, n * sizeof(unsigned)));
-        if (ws.counters) ws.retired.push_back(ws.counters);
-        ws.counters = (unsigned *)buf;
-        ws.counter_cap = 0;
-        HIP_TRY(qmv::launch_fill_u32(ws.counters, n, 0u, stream));
-        ws.counter_cap = n;
-    }
+    const size_t n = bytes + bytes / 4;
+    void *buf = nullptr;
+    HIP_TRY(qmv::shim_malloc(&buf, n));
+    if (ws.data) ws.retired.push_back(ws.data);
+    ws.data = (unsigned char *)buf;
+    ws.cap = n;
     return 1;
 }
 
@@ -239,10 +225,11 @@ int attend(qmv::AttnParams &p, int type, hipStream_t stream)
     }
     Workspace &ws = workspace_for(device, stream);
     std::lock_guard<std::mutex> lock(ws.mu);
-    if (!workspace_reserve(ws, stream, plan.partials, plan.counters)) return 0;
+    const size_t partial_bytes = plan.partials * sizeof(float);
+    if (!workspace_reserve(ws, stream, partial_bytes + plan.joins)) return 0;
     p.target = plan.target;
-    p.partials = ws.partials;
-    p.counters = ws.counters;
+    p.partials = (float *)ws.data;
+    p.joins = (qmv::AttnJoin *)(ws.data + partial_bytes);
     HIP_TRY(qmv::launch_attention(p, plan, type, stream));
     return 1;
 }

@@ -161,6 +161,7 @@ struct AttnTokens {
     int *status; /* may be null */
 };
 
+struct AttnJoin;
 struct AttnParams {
     AttnTokens t;
     const float *q;
@@ -171,8 +172,8 @@ struct AttnParams {
     /* Work of few rows is cut along the keys into about `target` pieces (0:
      * not), whose partial results meet in the workspace. */
     int target;
-    float *partials;    /* attn_partial_floats() for each workgroup */
-    unsigned *counters; /* one per row tile and key head, zero between launches */
+    float *partials;
+    AttnJoin *joins; /* [0].n: row tiles in all; [1 + tile] */
 };
 
 /* How a call is launched: rows (token, head of the group) per workgroup, the
@@ -182,7 +183,7 @@ struct AttnPlan {
     int target;
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
-    size_t partials, counters; /* floats, words */
+    size_t partials, joins; /* floats, bytes */
 };
 
 struct RopeParams {
