@@ -207,6 +207,80 @@ __device__ __forceinline__ void limbs_of(const float *x, float by, h8_t *hi, h8_
 __device__ const u4_t kNoPiece[4] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {~0u, ~0u, ~0u, ~0u}, {~0u, ~0u, ~0u, ~0u}};
 constexpr int64_t kPastEnd = -2, kNoPage = -1;
 
+/* Pieces of 8 elements that a lane loads, as 16-byte words. */
+template <int TYPE> struct Raw {
+    static constexpr int WORDS = TYPE == QMV_KV_F32 ? 2 : 1;
+    static constexpr uint32_t INF = TYPE == QMV_KV_F32 ? 0x7f800000u : TYPE == QMV_KV_F16 ? 0x7c00u : 0x7f80u;
+    u4_t w[WORDS];
+
+    /* The largest finite magnitude's bits (f16, bf16: its code) and whether any
+     * element is not finite. */
+    __device__ __forceinline__ void look(uint32_t *top, bool *odd) const
+    {
+#pragma unroll
+        for (int i = 0; i < 4 * WORDS; ++i) {
+            const uint32_t x = w[i >> 2][i & 3];
+            if (TYPE == QMV_KV_F32) {
+                const uint32_t m = x & 0x7fffffffu;
+                *odd |= m >= INF;
+                *top = max(*top, m >= INF ? 0u : m);
+            } else {
+                const uint32_t m0 = x & 0x7fffu, m1 = x >> 16 & 0x7fffu;
+                *odd |= m0 >= INF || m1 >= INF;
+                *top = max(*top, max(m0 >= INF ? 0u : m0, m1 >= INF ? 0u : m1));
+            }
+        }
+    }
+
+    /* f(element) for those that are not finite, which become zero. */
+    template <typename F> __device__ __forceinline__ void clear_odd(F f)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            constexpr bool wide = TYPE == QMV_KV_F32;
+            const uint32_t x = w[wide ? e >> 2 : 0][wide ? e & 3 : e >> 1];
+            const uint32_t mask = wide ? INF : INF << 16 * (e & 1);
+            if ((x & mask) == mask) {
+                w[wide ? e >> 2 : 0][wide ? e & 3 : e >> 1] = wide ? 0u : x & 0xffff0000u >> 16 * (e & 1);
+                f(e);
+            }
+        }
+    }
+
+    /* As f16 limbs, after a factor 2^n (not of f16), to `to` and to + apart. */
+    __device__ __forceinline__ void put(unsigned char *to, int apart, int n) const
+    {
+        if (TYPE == QMV_KV_F16) {
+            *(u4_t *)to = w[0];
+        } else if (TYPE == QMV_KV_BF16) {
+            h8_t h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[2 * e] = (_Float16)(__uint_as_float(w[0][e] << 16) * power_of_two(n));
+                h[2 * e + 1] = (_Float16)(__uint_as_float(w[0][e] & 0xffff0000u) * power_of_two(n));
+            }
+            *(h8_t *)to = h;
+        } else {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e >> 2][e & 3]);
+            h8_t hi, lo;
+            limbs_of(x, power_of_two(n), &hi, &lo);
+            *(h8_t *)to = hi;
+            *(h8_t *)(to + apart) = lo;
+        }
+    }
+};
+
+/* A tile in LDS is rows of keys. Piece c of a key is at place c ^ turn(key):
+ * neither the loads of one piece of many keys nor the transposing loads of a
+ * few pieces of four keys meet in a bank. */
+template <int DP> __device__ __forceinline__ int turn_of(int key)
+{
+    return DP == 128 ? (key & 3) << 2 | (key >> 2 & 3) : (key >> 1 & 1) << 2 | (key >> 2 & 3);
+}
+constexpr int kMostKeys = 126, kMostValues = 100; /* most factors of scale_of */
+
 struct AttnItem {
     int s, start, n, len; /* the sequence, its first token, new tokens and length (cut to its pages) */
     int first;            /* position of its first new token */
@@ -289,10 +363,77 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     return found;
 }
 
+/* Long prompts: their keys and values are split into limbs once, as images of
+ * the tiles in LDS: K high, K low, V high, V low, and a head of floats: the
+ * blocks' factors of the keys, exponents of the values, and whether any value
+ * is not finite. Sequence s has its tiles from start / 64 + s on. */
+constexpr int kImageKeys = 64, kImageHead = 64;
+__host__ __device__ constexpr int64_t image_bytes(int dp) { return kImageKeys * dp * 2 * 4 + kImageHead * 4; }
+
+template <int DP> __global__ __launch_bounds__(256) void attention_image_kernel(AttnParams p)
+{
+    constexpr int SLOTS = DP / 32, PIECES = DP / 8, PER = 64 / PIECES, MAT = kImageKeys * DP * 2;
+    __shared__ int odd_waves[4];
+    const AttnTokens &a = p.t;
+    const int lane = threadIdx.x & 63, b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); /* a block of 16 keys */
+    const int kvh = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads;
+    auto start_of = [&](int s) { return min(max(a.starts[s], 0), a.tokens); };
+    int lo = 0, hi = a.count; /* the last sequence that begins at this tile or before */
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start_of(mid) / kImageKeys + mid <= at) lo = mid;
+        else hi = mid;
+    }
+    const int start = start_of(lo), n = start_of(lo + 1) - start, first = (at - start / kImageKeys - lo) * kImageKeys;
+    if (first < 0 || first >= n) return;
+    unsigned char *const image = p.image + (int64_t)blockIdx.x * image_bytes(DP);
+    float *const head = (float *)(image + 4 * MAT);
+    const int piece = lane % PIECES, sub = lane / PIECES;
+    Raw<QMV_KV_F32> raw[2][SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+        const int j = first + 16 * b + i * PER + sub;
+        const bool there = j < n && 8 * piece < a.dim;
+        const int64_t column = (int64_t)kvh * a.dim + 8 * piece;
+        const u4_t *k = there ? (const u4_t *)((const float *)p.k + (start + j) * p.k_stride + column) : kNoPiece;
+        const u4_t *v = there ? (const u4_t *)((const float *)p.v + (start + j) * p.v_stride + column) : kNoPiece;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            raw[0][i].w[r] = k[r];
+            raw[1][i].w[r] = v[r];
+        }
+    }
+    bool odd_values = false;
+#pragma unroll
+    for (int values = 0; values < 2; ++values) {
+        uint32_t top = 0;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) raw[values][i].look(&top, &odd);
+        const int n2 = scale_of(wave_max(top), values ? kMostValues : kMostKeys);
+        if (lane == 0) head[4 * values + b] = values ? (float)-n2 : power_of_two(-n2);
+        if (values && __any(odd)) {
+            odd_values = true;
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) raw[1][i].clear_odd([](int) {});
+        }
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            const int key = i * PER + sub;
+            raw[values][i].put(image + 2 * values * MAT + (16 * b + key) * DP * 2 + ((piece ^ turn_of<DP>(key)) << 4), MAT, n2);
+        }
+    }
+    if (lane == 0) odd_waves[b] = odd_values;
+    __syncthreads();
+    if (threadIdx.x < kImageHead - 8)
+        head[8 + threadIdx.x] = threadIdx.x == 4 && (odd_waves[0] | odd_waves[1] | odd_waves[2] | odd_waves[3]) ? 1.f : 0.f;
+}
+
 /* DP: head_dim padded to 64 or 128; RW: rows of a wave; WR waves along the
  * rows, WK along the keys. */
 template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
-    static constexpr int NL = TYPE == QMV_KV_F32 ? 2 : 1;   /* limbs of keys and values */
+    static constexpr bool IMAGE = TYPE == QMV_KV_IMAGE;
+    static constexpr int NL = TYPE == QMV_KV_F32 || IMAGE ? 2 : 1; /* limbs of keys and values */
     static constexpr int KT = WR >= 4 ? 64 : 32;            /* keys a wave takes per tile */
     static constexpr int NB = KT / 16;                      /* blocks of 16 keys */
     static constexpr int UNITS = 2 * NB / WR;               /* blocks (of keys, of values) a wave loads */
@@ -301,7 +442,8 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int TILE = 2 * NL * MAT;
     static constexpr int ROWS = RW * WR;
     static constexpr int JOIN = WK > 1 ? WK * (RW * DP * 4) : 0; /* the waves' O, where they meet */
-    static constexpr int LDS = WK * TILE > JOIN ? WK * TILE : JOIN;
+    static constexpr int TILES = IMAGE ? 2 : WK;
+    static constexpr int LDS = TILES * TILE > JOIN ? TILES * TILE : JOIN;
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
 };
 
@@ -311,11 +453,13 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
     using P = Product<RW>;
     using acc_t = typename P::acc_t;
+    constexpr bool IMAGE = S::IMAGE;
     constexpr int KT = S::KT, NB = S::NB, UNITS = S::UNITS, SLOTS = S::SLOTS, MAT = S::MAT, NL = S::NL;
     constexpr int THREADS = 64 * WR * WK, WIDE = 512 / RW; /* of a product's contraction */
     constexpr int STEPS = DP / WIDE, DB = DP / RW, REGS = RW * RW / 64, SCORES = RW / 2;
     __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
-    __shared__ float scales[WK][2 * NB]; /* of the keys: factors; of the values: exponents */
+    /* of the keys: factors; of the values: exponents; of an image: its whole head */
+    __shared__ float scales[S::TILES][IMAGE ? kImageHead : 2 * NB];
     __shared__ int first_odd[DP]; /* the first key whose value is not finite there */
     __shared__ int any_odd;
     __shared__ float joined[WK > 1 ? WK : 1][2][RW];
@@ -352,7 +496,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     const bool real = token < it.n;
     const int pos = real ? it.first + token : -1;
     /* ---- tiles: loads into registers, then as f16 limbs into LDS ---- */
-    unsigned char *const tile = lds + wk * S::TILE;
+    unsigned char *tile = lds + (IMAGE ? 0 : wk * S::TILE);
+    int buf = IMAGE ? 0 : wk;
     constexpr int PIECES = DP / 8, PER = 64 / PIECES; /* of a key; keys per slot */
     const int piece = lane % PIECES, sub = lane / PIECES;
     constexpr int OWN = WR == 1 ? KT : 16; /* keys whose places a wave looks up */
@@ -366,8 +511,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         if (at < 0 && a.status) *a.status = 0;
         return at;
     };
-    constexpr int RAW = TYPE == QMV_KV_F32 ? 2 : 1; /* 16-byte loads per piece */
-    u4_t raw[UNITS][SLOTS][RAW];
+    Raw<TYPE> raw[UNITS][SLOTS];
     auto unit_block = [&](int u) { return WR == 1 ? u % NB : wr % NB; };
     auto unit_values = [&](int u) { return WR == 1 ? u >= NB : UNITS == 1 ? wr >= NB : u == 1; };
     auto load = [&](int64_t at) {
@@ -381,7 +525,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                 if (from < 0 || 8 * piece >= dim)
                     src = (const unsigned char *)(kNoPiece + (from == kNoPage && !unit_values(u) && 8 * piece < dim ? 2 : 0));
 #pragma unroll
-                for (int r = 0; r < RAW; ++r) raw[u][i][r] = ((const u4_t *)src)[r];
+                for (int r = 0; r < Raw<TYPE>::WORDS; ++r) raw[u][i].w[r] = ((const u4_t *)src)[r];
             }
         }
     };
@@ -391,29 +535,12 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         for (int u = 0; u < UNITS; ++u) {
             const int b = unit_block(u);
             const bool values = unit_values(u);
-            unsigned char *to = tile + (values ? NL * MAT : 0) + 16 * b * DP * 2;
-            uint32_t top = 0; /* the largest magnitude, bits of fp32 (f16, bf16: of two codes) */
             int n = 0;
             if (TYPE != QMV_KV_F16 || (values && masked)) {
-                constexpr uint32_t inf = TYPE == QMV_KV_F32 ? 0x7f800000u : TYPE == QMV_KV_F16 ? 0x7c00u : 0x7f80u;
+                uint32_t top = 0;
                 bool odd = false;
 #pragma unroll
-                for (int i = 0; i < SLOTS; ++i)
-#pragma unroll
-                    for (int r = 0; r < RAW; ++r)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t w = raw[u][i][r][e];
-                            if (TYPE == QMV_KV_F32) {
-                                const uint32_t m = w & 0x7fffffffu;
-                                odd |= m >= inf;
-                                top = max(top, m >= inf ? 0u : m);
-                            } else {
-                                const uint32_t m0 = w & 0x7fffu, m1 = w >> 16 & 0x7fffu;
-                                odd |= m0 >= inf || m1 >= inf;
-                                top = max(top, max(m0 >= inf ? 0u : m0, m1 >= inf ? 0u : m1));
-                            }
-                        }
+                for (int i = 0; i < SLOTS; ++i) raw[u][i].look(&top, &odd);
                 /* A value that is not finite must not reach the rows that do not
                  * attend it, and 0 * inf is NaN: where some do not, zero takes its
                  * place here, and the rows that do are marked at the end. */
@@ -421,56 +548,47 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                     if (lane == 0) any_odd = 1;
 #pragma unroll
                     for (int i = 0; i < SLOTS; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            constexpr bool wide = TYPE == QMV_KV_F32;
-                            const uint32_t w = raw[u][i][wide ? e >> 2 : 0][wide ? e & 3 : e >> 1];
-                            const uint32_t mask = wide ? inf : inf << 16 * (e & 1);
-                            if ((w & mask) == mask) {
-                                raw[u][i][wide ? e >> 2 : 0][wide ? e & 3 : e >> 1] = wide ? 0u : w & 0xffff0000u >> 16 * (e & 1);
-                                atomicMin(&first_odd[8 * piece + e], k0 + 16 * b + i * PER + sub);
-                            }
-                        }
+                        raw[u][i].clear_odd([&](int e) { atomicMin(&first_odd[8 * piece + e], k0 + 16 * b + i * PER + sub); });
                 }
                 if (TYPE != QMV_KV_F16) {
                     top = wave_max(top);
-                    n = scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? 100 : 126);
+                    n = scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? kMostValues : kMostKeys);
                     if (lane == 0) scales[wk][values ? NB + b : b] = values ? (float)-n : power_of_two(-n);
                 }
             }
+            unsigned char *to = tile + (values ? NL * MAT : 0) + 16 * b * DP * 2;
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) {
-                const int r = i * PER + sub;
-                const int turn = DP == 128 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3);
-                unsigned char *at = to + r * DP * 2 + ((piece ^ turn) << 4);
-                if (TYPE == QMV_KV_F16) {
-                    *(u4_t *)at = raw[u][i][0];
-                } else if (TYPE == QMV_KV_BF16) {
-                    h8_t h;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        h[2 * e] = (_Float16)(__uint_as_float(raw[u][i][0][e] << 16) * power_of_two(n));
-                        h[2 * e + 1] = (_Float16)(__uint_as_float(raw[u][i][0][e] & 0xffff0000u) * power_of_two(n));
-                    }
-                    *(h8_t *)at = h;
-                } else {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[u][i][e >> 2][e & 3]);
-                    h8_t hi, lo;
-                    limbs_of(x, power_of_two(n), &hi, &lo);
-                    *(h8_t *)at = hi;
-                    *(h8_t *)(at + MAT) = lo;
-                }
+                const int key = i * PER + sub;
+                raw[u][i].put(to + key * DP * 2 + ((piece ^ turn_of<DP>(key)) << 4), MAT, n);
             }
         }
     };
 
+    /* An image's tile goes to LDS as it is. */
+    const int64_t image_at = IMAGE ? it.start / KT + it.s : 0;
+    auto fetch = [&](int k0, int buf) {
+        constexpr int MINE = S::TILE / (WR * WK);
+        const unsigned char *src = p.image + ((image_at + k0 / KT) * a.kv_heads + kvh) * image_bytes(DP);
+        unsigned char *to = lds + buf * S::TILE + wave * MINE;
+        typedef __attribute__((address_space(1))) void *from_t;
+        typedef QMV_LDS void *to_t;
+#pragma unroll
+        for (int i = 0; i < MINE; i += 1024)
+            __builtin_amdgcn_global_load_lds((from_t)(src + wave * MINE + i + lane * 16), (to_t)(to + i), 16, 0, 0);
+        if (wave == 0) __builtin_amdgcn_global_load_lds((from_t)(src + S::TILE + lane * 4), (to_t)&scales[buf][0], 4, 0, 0);
+    };
+
     constexpr int STEP = KT * WK;
     int k0 = begin + wk * KT;
-    int64_t next = place(k0);
-    if (begin < end) load(next);
-    next = place(k0 + STEP);
+    int64_t next = 0;
+    if constexpr (IMAGE) {
+        if (begin < end) fetch(begin, 0);
+    } else {
+        next = place(k0);
+        if (begin < end) load(next);
+        next = place(k0 + STEP);
+    }
 
     /* q as two limbs, 8 elements of each step */
     h8_t qhi[STEPS], qlo[STEPS];
@@ -508,8 +626,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     float r = kNothing, l = 0.f;
     /* Key 32 sb + score_key(i) of a tile is the one of score register i. */
     auto score_key = [&](int i) { return (256 / RW) * (i >> 2) + 4 * part_of + (i & 3); };
-    const int turn_k = DP == 128 ? (col & 3) << 2 | (col >> 2 & 3) : (col >> 1 & 1) << 2 | (col >> 2 & 3);
-    const int k_at = col * DP * 2 + ((part_of ^ turn_k) << 4);
+    const int k_at = col * DP * 2 + ((part_of ^ turn_of<DP>(col)) << 4);
     /* K of RW keys, one step of the contraction. */
     auto k_frag = [&](int limb, int kb, int st) -> h8_t {
         return *(const h8_t *)(tile + limb * MAT + kb * RW * DP * 2 + (k_at ^ st * (WIDE * 2)));
@@ -519,9 +636,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int key = 256 / RW * i + 4 * part_of + kk;
-        const int turn = DP == 128 ? kk << 2 | (key >> 2 & 3) : (kk >> 1) << 2 | (key >> 2 & 3);
         const int at = (RW == 32 ? (lane >> 4 & 1) << 1 : 0) | (lane >> 1 & 1); /* pieces within the product's rows */
-        v_at[i] = key * DP * 2 + ((at ^ turn) << 4) + (lane & 1) * 8;
+        v_at[i] = key * DP * 2 + ((at ^ turn_of<DP>(key)) << 4) + (lane & 1) * 8;
     }
     /* V^T of one step of keys and RW elements: 8 keys of one element a lane, in
      * the order in which the scores are in its registers. */
@@ -567,8 +683,8 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
                     add[g] = 0.f;
                 } else {
                     /* within the finite positive floats, so that a masked score stays -inf */
-                    by[g] = fminf(fmaxf(q_back * scales[wk][2 * sb + g], 1.1754944e-38f), 1.7014118e38f);
-                    add[g] = scales[wk][NB + 2 * sb + g];
+                    by[g] = fminf(fmaxf(q_back * scales[buf][2 * sb + g], 1.1754944e-38f), 1.7014118e38f);
+                    add[g] = scales[buf][NB + 2 * sb + g];
                     back[g] = __builtin_ldexpf(1.f, -20 - (int)add[g]); /* may be a denormal */
                 }
                 constexpr int EACH = SCORES / 2; /* scores of a block of 16 keys */
@@ -614,15 +730,36 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         }
     };
 
-    for (int at = begin; at < end; at += STEP, k0 += STEP) {
-        if (WR > 1) lds_barrier(); /* the last tile has been read */
-        store(k0);
-        if (at + STEP < end) load(next);
-        next = place(k0 + 2 * STEP);
-        if (WR > 1) lds_barrier();
-        else asm volatile("" ::: "memory");
-        if (k0 < end) compute(k0);
-        if (WR == 1) asm volatile("" ::: "memory");
+    if constexpr (IMAGE) {
+        for (; k0 < end; k0 += STEP) {
+            __builtin_amdgcn_s_waitcnt(0x0F70); /* vmcnt(0): this wave's part of the tile */
+            lds_barrier();                      /* and the others'; the tile before has been read */
+            if (k0 + STEP < end) fetch(k0 + STEP, buf ^ 1);
+            if (scales[buf][3 * NB] != 0.f) { /* values that are not finite, zeros in the image */
+                any_odd = 1;
+                for (int i = tid; i < KT * dim; i += THREADS) {
+                    const int j = k0 + i / dim, d = i % dim;
+                    if (j >= it.n) break;
+                    const float x = ((const float *)p.v)[(it.start + j) * p.v_stride + (int64_t)kvh * dim + d];
+                    if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) atomicMin(&first_odd[d], j);
+                }
+            }
+            compute(k0);
+            buf ^= 1;
+            tile = lds + buf * S::TILE;
+        }
+        lds_barrier();
+    } else {
+        for (int at = begin; at < end; at += STEP, k0 += STEP) {
+            if (WR > 1) lds_barrier(); /* the last tile has been read */
+            store(k0);
+            if (at + STEP < end) load(next);
+            next = place(k0 + 2 * STEP);
+            if (WR > 1) lds_barrier();
+            else asm volatile("" ::: "memory");
+            if (k0 < end) compute(k0);
+            if (WR == 1) asm volatile("" ::: "memory");
+        }
     }
     l = sum_lanes<RW>(l);
     constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
@@ -805,6 +942,10 @@ AttnPlan plan_attention(const AttnTokens &t)
         plan.joins = (1 + (size_t)tiles) * sizeof(AttnJoin);
         plan.partials = (size_t)plan.grid * (plan.rows * (dp + 2));
     }
+    if (plan.rows == 256 && t.page_size == 0) {
+        plan.images = ((int64_t)t.tokens / kImageKeys + t.count) * t.kv_heads;
+        plan.image_bytes = (size_t)(plan.images * image_bytes(t.dim <= 64 ? 64 : 128));
+    }
     return plan;
 }
 
@@ -825,6 +966,13 @@ template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const A
     else launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
 }
 
+/* A prompt's rows of fp32, through images of their tiles. */
+template <int DP> static void launch_images(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+{
+    attention_image_kernel<DP><<<dim3((unsigned)plan.images), 256, 0, s>>>(p);
+    launch_shape<QMV_KV_IMAGE, DP, 32, 8, 1>(p, plan, s);
+}
+
 template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     if (p.t.dim <= 64) launch_rows<TYPE, 64>(p, plan, s);
@@ -833,7 +981,10 @@ template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &
 
 hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s)
 {
-    if (type == QMV_KV_F32) launch_dim<QMV_KV_F32>(p, plan, s);
+    if (plan.images) {
+        if (p.t.dim <= 64) launch_images<64>(p, plan, s);
+        else launch_images<128>(p, plan, s);
+    } else if (type == QMV_KV_F32) launch_dim<QMV_KV_F32>(p, plan, s);
     else if (type == QMV_KV_F16) launch_dim<QMV_KV_F16>(p, plan, s);
     else launch_dim<QMV_KV_BF16>(p, plan, s);
     return hipGetLastError();

@@ -226,10 +226,11 @@ int attend(qmv::AttnParams &p, int type, hipStream_t stream)
     Workspace &ws = workspace_for(device, stream);
     std::lock_guard<std::mutex> lock(ws.mu);
     const size_t partial_bytes = plan.partials * sizeof(float);
-    if (!workspace_reserve(ws, stream, partial_bytes + plan.joins)) return 0;
+    if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + plan.joins)) return 0;
     p.target = plan.target;
-    p.partials = (float *)ws.data;
-    p.joins = (qmv::AttnJoin *)(ws.data + partial_bytes);
+    p.image = ws.data;
+    p.partials = (float *)(ws.data + plan.image_bytes);
+    p.joins = (qmv::AttnJoin *)(ws.data + plan.image_bytes + partial_bytes);
     HIP_TRY(qmv::launch_attention(p, plan, type, stream));
     return 1;
 }
@@ -349,6 +350,8 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
     p.v = d_v;
     p.out = d_out;
     p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
     p.out_stride = out_stride;
     p.scale = scale;
     return attend(p, QMV_KV_F32, (hipStream_t)stream);

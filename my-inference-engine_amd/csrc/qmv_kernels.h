@@ -168,11 +168,13 @@ struct AttnParams {
     const void *k, *v;
     float *out;
     int64_t q_stride, out_stride;
+    int64_t k_stride, v_stride; /* of a prompt's rows */
     float scale;
     /* Work of few rows is cut along the keys into about `target` pieces (0:
      * not), whose partial results meet in the workspace. */
     int target;
     float *partials;
+    unsigned char *image; /* a prompt's keys and values as tiles of limbs */
     AttnJoin *joins; /* [0].n: row tiles in all; [1 + tile] */
 };
 
@@ -184,6 +186,8 @@ struct AttnPlan {
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
     size_t partials, joins; /* floats, bytes */
+    int64_t images;         /* tiles that are made first, 0: none */
+    size_t image_bytes;
 };
 
 struct RopeParams {
@@ -200,6 +204,7 @@ struct RopeParams {
 #define QMV_KV_F32 0
 #define QMV_KV_F16 1
 #define QMV_KV_BF16 2
+#define QMV_KV_IMAGE 3
 AttnPlan plan_attention(const AttnTokens &t);
 hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s);
 hipError_t launch_rope(const RopeParams &p, int type, hipStream_t s);
