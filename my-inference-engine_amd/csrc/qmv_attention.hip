@@ -190,15 +190,20 @@ __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((u
  * `most`. */
 __device__ __forceinline__ int scale_of(uint32_t bits, int most) { return min(14 - ((int)(bits >> 23) - 127), most); }
 
-/* Eight values as two limbs. */
-__device__ __forceinline__ void limbs_of(const float *x, float by, h8_t *hi, h8_t *lo)
+/* Eight values as two limbs. In pairs, so that a limb is rounded once, packed;
+ * v - hi is one instruction as a multiply-add of a half and a float. */
+__device__ __forceinline__ void limbs_of(const float *x, h8_t *hi, h8_t *lo)
 {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = x[i] * by;
-        const _Float16 h = (_Float16)v;
-        (*hi)[i] = h;
-        (*lo)[i] = (_Float16)(v - (float)h);
+    for (int i = 0; i < 8; i += 2) {
+        const f2_t v = {x[i], x[i + 1]};
+        const h2_t h = __builtin_convertvector(v, h2_t);
+        const f2_t rest = {fmaf((float)h[0], -1.f, v[0]), fmaf((float)h[1], -1.f, v[1])};
+        const h2_t l = __builtin_convertvector(rest, h2_t);
+        (*hi)[i] = h[0];
+        (*hi)[i + 1] = h[1];
+        (*lo)[i] = l[0];
+        (*lo)[i + 1] = l[1];
     }
 }
 
@@ -213,23 +218,33 @@ template <int TYPE> struct Raw {
     static constexpr uint32_t INF = TYPE == QMV_KV_F32 ? 0x7f800000u : TYPE == QMV_KV_F16 ? 0x7c00u : 0x7f80u;
     u4_t w[WORDS];
 
-    /* The largest finite magnitude's bits (f16, bf16: its code) and whether any
+    /* The largest magnitude's bits (f16, bf16: its code); at least INF where an
      * element is not finite. */
-    __device__ __forceinline__ void look(uint32_t *top, bool *odd) const
+    __device__ __forceinline__ uint32_t top() const
     {
+        uint32_t m = 0;
+        if (TYPE == QMV_KV_F32) {
 #pragma unroll
-        for (int i = 0; i < 4 * WORDS; ++i) {
-            const uint32_t x = w[i >> 2][i & 3];
-            if (TYPE == QMV_KV_F32) {
-                const uint32_t m = x & 0x7fffffffu;
-                *odd |= m >= INF;
-                *top = max(*top, m >= INF ? 0u : m);
-            } else {
-                const uint32_t m0 = x & 0x7fffu, m1 = x >> 16 & 0x7fffu;
-                *odd |= m0 >= INF || m1 >= INF;
-                *top = max(*top, max(m0 >= INF ? 0u : m0, m1 >= INF ? 0u : m1));
-            }
+            for (int i = 0; i < 8; ++i) m = max(m, w[i >> 2][i & 3] & 0x7fffffffu);
+            return m;
         }
+        typedef uint16_t s2_t __attribute__((ext_vector_type(2)));
+        s2_t m2 = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(s2_t, w[0][i] & 0x7fff7fffu));
+        return max(m2[0], m2[1]);
+    }
+
+    /* The same of the finite ones. */
+    __device__ __forceinline__ uint32_t top_finite() const
+    {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t x = TYPE == QMV_KV_F32 ? w[i >> 2][i & 3] & 0x7fffffffu : w[0][i >> 1] >> 16 * (i & 1) & 0x7fffu;
+            m = max(m, x >= INF ? 0u : x);
+        }
+        return m;
     }
 
     /* f(element) for those that are not finite, which become zero. */
@@ -256,16 +271,19 @@ template <int TYPE> struct Raw {
             h8_t h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                h[2 * e] = (_Float16)(__uint_as_float(w[0][e] << 16) * power_of_two(n));
-                h[2 * e + 1] = (_Float16)(__uint_as_float(w[0][e] & 0xffff0000u) * power_of_two(n));
+                const f2_t v = {__uint_as_float(w[0][e] << 16) * power_of_two(n),
+                                __uint_as_float(w[0][e] & 0xffff0000u) * power_of_two(n)};
+                const h2_t h2 = __builtin_convertvector(v, h2_t);
+                h[2 * e] = h2[0];
+                h[2 * e + 1] = h2[1];
             }
             *(h8_t *)to = h;
         } else {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e >> 2][e & 3]);
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e >> 2][e & 3]) * power_of_two(n);
             h8_t hi, lo;
-            limbs_of(x, power_of_two(n), &hi, &lo);
+            limbs_of(x, &hi, &lo);
             *(h8_t *)to = hi;
             *(h8_t *)(to + apart) = lo;
         }
@@ -317,20 +335,24 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
         if (len > room) len = room + 1; /* one key past the table: its rows are NaN */
         tiles = (n * group + BM - 1) / BM;
     };
-    float work = 0.f, rows = 0.f;
+    float work = 0.f, rows = 0.f, tiles_sum = 0.f;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         read(s0 + lane);
         work += (float)tiles * (float)len;
         rows += (float)n;
+        tiles_sum += (float)tiles;
     }
     work = lane_of(scan_lanes(work), 63);
     rows = lane_of(scan_lanes(rows), 63);
+    tiles_sum = lane_of(scan_lanes(tiles_sum), 63);
     *tiles_all = 0;
     if (rows > (float)a.tokens) return false;
     int chunk = INT32_MAX / STEP * STEP;
     if (p.target) {
-        const float each = work / (float)max(p.target / a.kv_heads, 1);
-        chunk = each < 1e9f ? max(((int)each + STEP) / STEP * STEP, 2 * STEP) : chunk;
+        /* pieces beside the tiles' last ones, which may be short */
+        const int pieces = p.target / a.kv_heads, tiles_in_all = (int)tiles_sum;
+        const float each = work / (float)max(max(pieces - tiles_in_all, pieces / 2), 1);
+        chunk = each < 1e9f ? max(((int)each + STEP) / STEP * STEP, p.least) : chunk;
     }
     int before = 0, tiles_before = 0;
     bool found = false;
@@ -407,16 +429,22 @@ template <int DP> __global__ __launch_bounds__(256) void attention_image_kernel(
 #pragma unroll
     for (int values = 0; values < 2; ++values) {
         uint32_t top = 0;
-        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < SLOTS; ++i) raw[values][i].look(&top, &odd);
-        const int n2 = scale_of(wave_max(top), values ? kMostValues : kMostKeys);
-        if (lane == 0) head[4 * values + b] = values ? (float)-n2 : power_of_two(-n2);
-        if (values && __any(odd)) {
-            odd_values = true;
+        for (int i = 0; i < SLOTS; ++i) top = max(top, raw[values][i].top());
+        top = wave_max(top);
+        if (top >= Raw<QMV_KV_F32>::INF) {
+            if (values) {
+                odd_values = true;
 #pragma unroll
-            for (int i = 0; i < SLOTS; ++i) raw[1][i].clear_odd([](int) {});
+                for (int i = 0; i < SLOTS; ++i) raw[1][i].clear_odd([](int) {});
+            }
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) top = max(top, raw[values][i].top_finite());
+            top = wave_max(top);
         }
+        const int n2 = scale_of(top, values ? kMostValues : kMostKeys);
+        if (lane == 0) head[4 * values + b] = values ? (float)-n2 : power_of_two(-n2);
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
             const int key = i * PER + sub;
@@ -538,20 +566,25 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             int n = 0;
             if (TYPE != QMV_KV_F16 || (values && masked)) {
                 uint32_t top = 0;
-                bool odd = false;
 #pragma unroll
-                for (int i = 0; i < SLOTS; ++i) raw[u][i].look(&top, &odd);
-                /* A value that is not finite must not reach the rows that do not
-                 * attend it, and 0 * inf is NaN: where some do not, zero takes its
-                 * place here, and the rows that do are marked at the end. */
-                if (values && masked && __any(odd)) {
-                    if (lane == 0) any_odd = 1;
+                for (int i = 0; i < SLOTS; ++i) top = max(top, raw[u][i].top());
+                top = wave_max(top);
+                if (top >= Raw<TYPE>::INF) {
+                    /* A value that is not finite must not reach the rows that do not
+                     * attend it, and 0 * inf is NaN: where some do not, zero takes
+                     * its place here, and the rows that do are marked at the end. */
+                    if (values && masked) {
+                        any_odd = 1;
 #pragma unroll
-                    for (int i = 0; i < SLOTS; ++i)
-                        raw[u][i].clear_odd([&](int e) { atomicMin(&first_odd[8 * piece + e], k0 + 16 * b + i * PER + sub); });
+                        for (int i = 0; i < SLOTS; ++i)
+                            raw[u][i].clear_odd([&](int e) { atomicMin(&first_odd[8 * piece + e], k0 + 16 * b + i * PER + sub); });
+                    }
+                    top = 0;
+#pragma unroll
+                    for (int i = 0; i < SLOTS; ++i) top = max(top, raw[u][i].top_finite());
+                    top = wave_max(top);
                 }
                 if (TYPE != QMV_KV_F16) {
-                    top = wave_max(top);
                     n = scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? kMostValues : kMostKeys);
                     if (lane == 0) scales[wk][values ? NB + b : b] = values ? (float)-n : power_of_two(-n);
                 }
@@ -616,7 +649,11 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
         const int n = scale_of(__float_as_uint(max_lanes<RW>(__uint_as_float(bits))), 126);
         q_back = power_of_two(-n);
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) limbs_of(x[st], power_of_two(n), &qhi[st], &qlo[st]);
+        for (int st = 0; st < STEPS; ++st) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[st][i] *= power_of_two(n);
+            limbs_of(x[st], &qhi[st], &qlo[st]);
+        }
     }
 
     /* ---- a tile's products ---- */
@@ -718,7 +755,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
             }
 #pragma unroll
             for (int g = 0; g < VS; ++g) {
-                limbs_of(w + 8 * g, 1.f, &phi[g], &plo[g]);
+                limbs_of(w + 8 * g, &phi[g], &plo[g]);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) {
                     const h8_t v = v_frag(0, VS * sb + g, db);
@@ -923,8 +960,23 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     }
 }
 
-#ifndef QMV_ATTN_TARGET
-#define QMV_ATTN_TARGET 512
+#ifndef QMV_T16
+#define QMV_T16 1024
+#endif
+#ifndef QMV_T32
+#define QMV_T32 512
+#endif
+#ifndef QMV_T128
+#define QMV_T128 512
+#endif
+#ifndef QMV_T256
+#define QMV_T256 256
+#endif
+#ifndef QMV_L16
+#define QMV_L16 128
+#endif
+#ifndef QMV_L128
+#define QMV_L128 128
 #endif
 AttnPlan plan_attention(const AttnTokens &t)
 {
@@ -934,7 +986,12 @@ AttnPlan plan_attention(const AttnTokens &t)
     plan.rows = each <= 16 ? 16 : each <= 48 ? 32 : each <= 1024 ? 128 : 256;
     const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
     plan.tiles = (int)tiles;
-    plan.target = tiles * t.kv_heads < 2048 ? QMV_ATTN_TARGET : 0;
+    /* As many pieces as fit the compute units at once, some more of the few-row
+     * kernel, whose sequences' lengths differ most. Prompts fill them with their
+     * tiles sooner. */
+    plan.target = plan.rows == 16 ? QMV_T16 : plan.rows == 32 ? QMV_T32 : plan.rows == 128 ? QMV_T128 : QMV_T256;
+    if (tiles * t.kv_heads >= (t.page_size ? 4096 : plan.target)) plan.target = 0;
+    plan.least = plan.rows <= 32 ? QMV_L16 : QMV_L128;
     const int64_t items = tiles + (plan.target ? plan.target / t.kv_heads + 1 : 0);
     plan.grid = items * t.kv_heads;
     if (plan.target) {
@@ -953,7 +1010,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
 {
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
-    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
+    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 4, EACH = 256 / (DP / 4 * GROUPS);
     const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * (ROWS / EACH));
     attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
 }

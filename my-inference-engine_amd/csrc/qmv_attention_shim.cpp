@@ -228,6 +228,7 @@ int attend(qmv::AttnParams &p, int type, hipStream_t stream)
     const size_t partial_bytes = plan.partials * sizeof(float);
     if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + plan.joins)) return 0;
     p.target = plan.target;
+    p.least = plan.least;
     p.image = ws.data;
     p.partials = (float *)(ws.data + plan.image_bytes);
     p.joins = (qmv::AttnJoin *)(ws.data + plan.image_bytes + partial_bytes);

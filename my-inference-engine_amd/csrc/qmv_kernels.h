@@ -173,6 +173,7 @@ struct AttnParams {
     /* Work of few rows is cut along the keys into about `target` pieces (0:
      * not), whose partial results meet in the workspace. */
     int target;
+    int least; /* keys of a piece at least, whole steps of the kernel */
     float *partials;
     unsigned char *image; /* a prompt's keys and values as tiles of limbs */
     AttnJoin *joins; /* [0].n: row tiles in all; [1 + tile] */
@@ -182,7 +183,7 @@ struct AttnParams {
  * workgroups and the workspace. */
 struct AttnPlan {
     int rows;
-    int target;
+    int target, least;
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
     size_t partials, joins; /* floats, bytes */
