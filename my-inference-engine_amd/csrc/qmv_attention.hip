@@ -338,7 +338,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     float work = 0.f, rows = 0.f, tiles_sum = 0.f;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         read(s0 + lane);
-        work += (float)tiles * (float)len;
+        work += (float)tiles * (a.page_size ? (float)len : 0.5f * (float)len); /* what the tiles attend, or more */
         rows += (float)n;
         tiles_sum += (float)tiles;
     }
@@ -371,7 +371,8 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
             out->n = lane_of(n, at);
             out->len = lane_of(len, at);
             out->first = lane_of(first, at);
-            out->chunk = chunk;
+            /* pieces of one length, not all but the last of `chunk` */
+            out->chunk = ((out->len + sp - 1) / sp + STEP - 1) / STEP * STEP;
             out->split = mine - nth * sp;
             out->tile = lane_of(tiles, at) - 1 - nth;
             out->tile_at = tiles_before + lane_of(tsum, at) - lane_of(tiles, at) + out->tile;
@@ -891,16 +892,16 @@ template <int DP, int ROWS, int GROUPS>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float down)
 {
     constexpr int D4 = DP / 4, EACH = 256 / (D4 * GROUPS); /* rows of a workgroup */
-    constexpr int AT_ONCE = 8;
+    constexpr int AT_ONCE = GROUPS > 1 ? 8 : 16;
     constexpr int PARTIAL = ROWS * DP + 2 * ROWS;
     __shared__ f4_t sums[GROUPS > 1 ? GROUPS : 1][EACH][D4];
     __shared__ f2_t states[GROUPS > 1 ? GROUPS : 1][EACH];
     const AttnTokens &a = p.t;
     const int slices = ROWS / EACH, group = a.heads / a.kv_heads;
     const int slice = blockIdx.x % slices, rest = blockIdx.x / slices, kvh = rest % a.kv_heads, tile_at = rest / a.kv_heads;
-    if (tile_at >= p.joins[0].n) return;
-    const AttnJoin j = p.joins[1 + tile_at];
-    if (j.pieces == 0) return;
+    const int tiles = p.joins[0].n;
+    const AttnJoin j = p.joins[1 + tile_at]; /* of no meaning past `tiles` */
+    if (tile_at >= tiles || j.pieces == 0) return;
     const int d4 = threadIdx.x % D4, set = threadIdx.x / D4 % GROUPS, rr = slice * EACH + threadIdx.x / (D4 * GROUPS);
     const int row = j.tile * ROWS + rr, token = row / group;
     if (j.tile * ROWS + slice * EACH >= j.n * group) return; /* no row of this workgroup */
@@ -960,6 +961,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     }
 }
 
+#ifndef QMV_IMG
+#define QMV_IMG 1024
+#endif
 #ifndef QMV_T16
 #define QMV_T16 1024
 #endif
@@ -972,34 +976,38 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
 #ifndef QMV_T256
 #define QMV_T256 256
 #endif
-#ifndef QMV_L16
-#define QMV_L16 128
+#ifndef QMV_T16F
+#define QMV_T16F 512
 #endif
-#ifndef QMV_L128
-#define QMV_L128 128
-#endif
-AttnPlan plan_attention(const AttnTokens &t)
+AttnPlan plan_attention(const AttnTokens &t, int type)
 {
     AttnPlan plan = {};
     const int group = t.heads / t.kv_heads;
     const int64_t rows = (int64_t)t.tokens * group, each = rows / t.count;
-    plan.rows = each <= 16 ? 16 : each <= 48 ? 32 : each <= 1024 ? 128 : 256;
+    plan.rows = each <= 16 ? 16 : each <= 48 ? 32 : each <= (t.dim <= 64 ? 4096 : 1024) ? 128 : 256;
     const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
     plan.tiles = (int)tiles;
     /* As many pieces as fit the compute units at once, some more of the few-row
      * kernel, whose sequences' lengths differ most. Prompts fill them with their
      * tiles sooner. */
-    plan.target = plan.rows == 16 ? QMV_T16 : plan.rows == 32 ? QMV_T32 : plan.rows == 128 ? QMV_T128 : QMV_T256;
+    plan.target = plan.rows == 16 ? (type == QMV_KV_F32 ? QMV_T16F : QMV_T16) : plan.rows == 32 ? QMV_T32 : plan.rows == 128 ? QMV_T128 : QMV_T256;
     if (tiles * t.kv_heads >= (t.page_size ? 4096 : plan.target)) plan.target = 0;
-    plan.least = plan.rows <= 32 ? QMV_L16 : QMV_L128;
-    const int64_t items = tiles + (plan.target ? plan.target / t.kv_heads + 1 : 0);
+    plan.least = plan.rows <= 32 && type != QMV_KV_F32 ? 256 : 128;
+    /* find_item's chunks cut all of the lengths' sum (of prompts, which attend
+     * half: half of it) into max(pieces - tiles, pieces / 2), and each tile has a
+     * last piece. Workgroups that find none cost their start, with the LDS of the
+     * others: 8 us of 21 where there were twice as many. */
+    const int64_t pieces = plan.target / t.kv_heads;
+    const int64_t items = plan.target == 0   ? tiles
+                          : t.page_size == 0 ? max(2 * pieces, pieces + tiles) + 1
+                                             : max(pieces, pieces / 2 + tiles) + 1;
     plan.grid = items * t.kv_heads;
     if (plan.target) {
         const int dp = t.dim <= 64 ? 64 : 128;
         plan.joins = (1 + (size_t)tiles) * sizeof(AttnJoin);
         plan.partials = (size_t)plan.grid * (plan.rows * (dp + 2));
     }
-    if (plan.rows == 256 && t.page_size == 0) {
+    if (plan.rows == 256 && t.page_size == 0 && t.tokens / t.count >= QMV_IMG) {
         plan.images = ((int64_t)t.tokens / kImageKeys + t.count) * t.kv_heads;
         plan.image_bytes = (size_t)(plan.images * image_bytes(t.dim <= 64 ? 64 : 128));
     }
@@ -1010,7 +1018,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
 {
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
-    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 4, EACH = 256 / (DP / 4 * GROUPS);
+    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
     const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * (ROWS / EACH));
     attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
 }

@@ -218,7 +218,7 @@ int attend(qmv::AttnParams &p, int type, hipStream_t stream)
 {
     const int device = qmv::shim_device();
     HIP_TRY(hipSetDevice(device));
-    const qmv::AttnPlan plan = qmv::plan_attention(p.t);
+    const qmv::AttnPlan plan = qmv::plan_attention(p.t, type);
     if (plan.grid > INT_MAX) {
         set_error("too many tokens and heads for one call");
         return 0;

@@ -206,7 +206,7 @@ struct RopeParams {
 #define QMV_KV_F16 1
 #define QMV_KV_BF16 2
 #define QMV_KV_IMAGE 3
-AttnPlan plan_attention(const AttnTokens &t);
+AttnPlan plan_attention(const AttnTokens &t, int type);
 hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s);
 hipError_t launch_rope(const RopeParams &p, int type, hipStream_t s);
 
