@@ -302,19 +302,23 @@ constexpr int kMostKeys = 126, kMostValues = 100; /* most factors of scale_of */
 struct AttnItem {
     int s, start, n, len; /* the sequence, its first token, new tokens and length (cut to its pages) */
     int first;            /* position of its first new token */
-    int tile, tile_at;    /* of its row tiles; among all sequences' */
+    int tiles;            /* its row tiles */
+    int tile, tile_at;    /* one of them; among all sequences' */
     int split, chunk;     /* keys [split * chunk, ...) */
 };
 
 /* What the pieces' join has to know of a row tile whose keys are cut. */
 struct AttnJoin {
     int start, n, tile; /* as in AttnItem */
-    int pieces, item;   /* how many, and which was the first; 0: not cut */
+    int pieces;         /* 0: not cut */
+    int item, apart;    /* the first piece's number, and what the next ones' are apart */
 };
 
-/* The `item`-th piece of a key head's work, by one wave: the sequences' row
- * tiles, the later ones (which attend more) first, each cut into pieces of
- * `chunk` keys. chunk is chosen here from all lengths, so that every workgroup
+/* The `item`-th piece of a key head's work, by one wave: of each sequence the
+ * first pieces of all row tiles, the later ones (which attend more) first, then
+ * their second pieces, and so on: consecutive workgroups run on different XCDs,
+ * and with a tile's pieces side by side those that have no keys were all on the
+ * same four (a prompt of 4096, 7B, 542 us in two pieces a tile). chunk is chosen here from all lengths, so that every workgroup
  * has the same; the sums are of floats, whose rounding the one piece beyond
  * plan_attention's count allows for. *tiles_all: row tiles in all, or 0 where
  * the starts fall so that there would be more rows than the call's. */
@@ -365,7 +369,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
         if (hit && !found) {
             const int at = __builtin_ctzll(hit);
             const int mine = item - before - (lane_of(sum, at) - lane_of(items, at));
-            const int sp = lane_of(splits, at), nth = mine / sp;
+            const int sp = lane_of(splits, at), all = lane_of(tiles, at), nth = mine % all;
             out->s = s0 + at;
             out->start = lane_of(start, at);
             out->n = lane_of(n, at);
@@ -373,9 +377,10 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
             out->first = lane_of(first, at);
             /* pieces of one length, not all but the last of `chunk` */
             out->chunk = ((out->len + sp - 1) / sp + STEP - 1) / STEP * STEP;
-            out->split = mine - nth * sp;
-            out->tile = lane_of(tiles, at) - 1 - nth;
-            out->tile_at = tiles_before + lane_of(tsum, at) - lane_of(tiles, at) + out->tile;
+            out->tiles = all;
+            out->split = mine / all;
+            out->tile = all - 1 - nth;
+            out->tile_at = tiles_before + lane_of(tsum, at) - all + out->tile;
             found = true;
         }
         before += lane_of(sum, 63);
@@ -477,7 +482,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
 };
 
 template <int TYPE, int DP, int RW, int WR, int WK>
-__global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
+__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1) void attention_kernel(AttnParams p)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
     using P = Product<RW>;
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(64 * WR * WK) void attention_kernel(AttnParams p)
     const int pieces = max((int)(((int64_t)keys + it.chunk - 1) / it.chunk), 1);
     if (it.split >= pieces) return;
     if (p.target && kvh == 0 && it.split == 0 && tid == 0)
-        p.joins[1 + it.tile_at] = AttnJoin{it.start, it.n, it.tile, pieces > 1 ? pieces : 0, item};
+        p.joins[1 + it.tile_at] = AttnJoin{it.start, it.n, it.tile, pieces > 1 ? pieces : 0, item, it.tiles};
     const int begin = it.split * it.chunk, end = min((int64_t)keys, (int64_t)begin + it.chunk);
     const int unmasked = it.first + it.tile * S::ROWS / group; /* every row attends keys up to here */
 
@@ -907,7 +912,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     if (j.tile * ROWS + slice * EACH >= j.n * group) return; /* no row of this workgroup */
     const bool real = token < j.n;
     const float *from = p.partials + ((int64_t)j.item * a.kv_heads + kvh) * PARTIAL;
-    const int64_t apart = (int64_t)a.kv_heads * PARTIAL;
+    const int64_t apart = (int64_t)j.apart * a.kv_heads * PARTIAL;
     const int mine = (j.pieces + GROUPS - 1) / GROUPS, i_end = min((set + 1) * mine, j.pieces);
     float all = kNothing, sum = 0.f;
     f4_t v = {0, 0, 0, 0};
@@ -967,15 +972,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
 #ifndef QMV_T16
 #define QMV_T16 1024
 #endif
-#ifndef QMV_T32
-#define QMV_T32 512
-#endif
 #ifndef QMV_T128
 #define QMV_T128 512
 #endif
 #ifndef QMV_T256
 #define QMV_T256 256
 #endif
+
 #ifndef QMV_T16F
 #define QMV_T16F 512
 #endif
@@ -984,15 +987,22 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     AttnPlan plan = {};
     const int group = t.heads / t.kv_heads;
     const int64_t rows = (int64_t)t.tokens * group, each = rows / t.count;
-    plan.rows = each <= 16 ? 16 : each <= 48 ? 32 : each <= (t.dim <= 64 ? 4096 : 1024) ? 128 : 256;
+    const int64_t room = t.page_size ? (int64_t)t.table_stride * t.page_size : t.tokens; /* keys at most */
+    const int64_t small = (rows / 16 + (t.count < t.tokens ? t.count : t.tokens)) * t.kv_heads;
+    plan.rows = each <= 16 || (small <= 256 && small * room <= 131072) ? 16 : each <= (t.dim <= 64 ? 4096 : type == QMV_KV_F32 ? 128 : 1024) ? 128 : 256;
+#ifdef QMV_FORCE
+    plan.rows = QMV_FORCE;
+#endif
     const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
     plan.tiles = (int)tiles;
     /* As many pieces as fit the compute units at once, some more of the few-row
      * kernel, whose sequences' lengths differ most. Prompts fill them with their
      * tiles sooner. */
-    plan.target = plan.rows == 16 ? (type == QMV_KV_F32 ? QMV_T16F : QMV_T16) : plan.rows == 32 ? QMV_T32 : plan.rows == 128 ? QMV_T128 : QMV_T256;
+    plan.target = plan.rows == 16 ? (type == QMV_KV_F32 ? QMV_T16F : QMV_T16) : plan.rows == 128 ? QMV_T128 : QMV_T256;
     if (tiles * t.kv_heads >= (t.page_size ? 4096 : plan.target)) plan.target = 0;
-    plan.least = plan.rows <= 32 && type != QMV_KV_F32 ? 256 : 128;
+    plan.least = plan.rows == 16 && type != QMV_KV_F32 ? 256 : 128;
+    /* what no sequence can have more of than one piece */
+    if (room <= plan.least) plan.target = 0;
     /* find_item's chunks cut all of the lengths' sum (of prompts, which attend
      * half: half of it) into max(pieces - tiles, pieces / 2), and each tile has a
      * last piece. Workgroups that find none cost their start, with the LDS of the
@@ -1018,7 +1028,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
 {
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
-    constexpr int ROWS = RW * WR, GROUPS = ROWS <= 32 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
+    constexpr int ROWS = RW * WR, GROUPS = ROWS == 16 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
     const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * (ROWS / EACH));
     attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
 }
@@ -1026,7 +1036,6 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     if (plan.rows == 16) launch_shape<TYPE, DP, 16, 1, 4>(p, plan, s);
-    else if (plan.rows == 32) launch_shape<TYPE, DP, 32, 1, 4>(p, plan, s);
     else if (plan.rows == 128) launch_shape<TYPE, DP, 32, 4, 1>(p, plan, s);
     else launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
 }
