@@ -427,7 +427,7 @@ int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q_heads,
  * grouped attention of src/transformer_ops.cpp:71):
  *   d_out[i] = sum_j softmax_j(scale * q_i . k_j) v_j
  * Rows as above (strides, alignment); sequences' lengths and pages are not
- * read. scale is finite. d_out overlaps no input.
+ * read. |scale| is at most 1e38. d_out overlaps no input.
  */
 int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride,
                                     const float *d_k, int64_t k_stride,

@@ -41,11 +41,9 @@ __device__ __forceinline__ int sequence_of(const AttnTokens &a, int t)
     return a.starts[lo + 1] > t ? lo : -1;
 }
 
-/* Where key `j` of sequence s (its first token is `start`) and of head h
- * begins, -1 if its page is outside the cache or the table. */
-__device__ __forceinline__ int64_t key_at(const AttnTokens &a, int s, int start, int j, int h)
+/* Where key `j` of sequence s and of head h begins in a paged cache, -1 if its page is outside the cache or the table. */
+__device__ __forceinline__ int64_t key_at(const AttnTokens &a, int s, int j, int h)
 {
-    if (a.page_size == 0) return (int64_t)(start + j) * a.token_stride + (int64_t)h * a.head_stride;
     const int page = j / a.page_size;
     if (page >= a.table_stride) return -1;
     const int at = a.table[(int64_t)s * a.table_stride + page];
@@ -376,7 +374,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
             out->len = lane_of(len, at);
             out->first = lane_of(first, at);
             /* pieces of one length, not all but the last of `chunk` */
-            out->chunk = ((out->len + sp - 1) / sp + STEP - 1) / STEP * STEP;
+            out->chunk = ((max(out->len, 1) + sp - 1) / sp + STEP - 1) / STEP * STEP;
             out->tiles = all;
             out->split = mine / all;
             out->tile = all - 1 - nth;
@@ -537,11 +535,13 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
     constexpr int OWN = WR == 1 ? KT : 16; /* keys whose places a wave looks up */
     const int own_first = WR == 1 ? 0 : 16 * (wr % NB);
 
-    /* Where lane's key (own_first + lane % OWN) of the tile at k0 begins. */
+    /* Where lane's key (own_first + lane % OWN) of the tile at k0 begins, of a
+     * prompt its row. */
     auto place = [&](int k0) -> int64_t {
         const int j = k0 + own_first + (lane & (OWN - 1));
         if (j >= end) return kPastEnd;
-        const int64_t at = key_at(a, it.s, it.start, j, kvh);
+        if (a.page_size == 0) return it.start + j;
+        const int64_t at = key_at(a, it.s, j, kvh);
         if (at < 0 && a.status) *a.status = 0;
         return at;
     };
@@ -554,7 +554,8 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
             const unsigned char *base = (const unsigned char *)(unit_values(u) ? p.v : p.k);
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) {
-                const int64_t from = shfl64(at, (WR == 1 ? 16 * unit_block(u) : 0) + i * PER + sub);
+                int64_t from = shfl64(at, (WR == 1 ? 16 * unit_block(u) : 0) + i * PER + sub);
+                if (a.page_size == 0 && from >= 0) from = from * (unit_values(u) ? p.v_stride : p.k_stride) + kvh * dim;
                 const unsigned char *src = base + (from + 8 * piece) * (TYPE == QMV_KV_F32 ? 4 : 2);
                 if (from < 0 || 8 * piece >= dim)
                     src = (const unsigned char *)(kNoPiece + (from == kNoPage && !unit_values(u) && 8 * piece < dim ? 2 : 0));
@@ -697,6 +698,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
         for (int sb = 0; sb < KT / 32; ++sb) {
             __builtin_amdgcn_sched_barrier(0);
             float c[SCORES];
+            __builtin_amdgcn_s_setprio(1); /* these products before the other waves' softmax: 1% of a long prompt */
 #pragma unroll
             for (int kb = 0; kb < 32 / RW; ++kb) {
                 acc_t x = {0};
@@ -710,6 +712,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
 #pragma unroll
                 for (int i = 0; i < REGS; ++i) c[REGS * kb + i] = x[i];
             }
+            __builtin_amdgcn_s_setprio(0);
             const int first = k0 + 32 * sb;
             const bool masked = first + 31 > unmasked;
             if (masked) {
@@ -966,60 +969,65 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     }
 }
 
-#ifndef QMV_IMG
-#define QMV_IMG 1024
-#endif
-#ifndef QMV_T16
-#define QMV_T16 1024
-#endif
-#ifndef QMV_T128
-#define QMV_T128 512
-#endif
-#ifndef QMV_T256
-#define QMV_T256 256
-#endif
-
-#ifndef QMV_T16F
-#define QMV_T16F 512
-#endif
+/* Rows per workgroup, by what was measured (us; 28 and 4 heads of 128, f16
+ * cache unless said, 16 / 128 / 256 rows):
+ *   16, where no sequence fills more, or where all tiles of 16 are one round of
+ *   the 256 compute units and the keys are few enough that reading them for
+ *   each tile costs less than the larger tiles' start: prompt of 37 tokens 10.9 /
+ *   13.2 / 16.4, of 128 11.5 / 18.4 / 21.7, of 256 28.8 / 25.4 / 28.9; 32 tokens
+ *   over 512 15.7 / 19.1 / 22.4, over 4096 32.8 / 28.0 / 30.2. (32 rows, tried,
+ *   were slower than 16 or than 128 at every size.)
+ *   256, one workgroup of 8 waves per compute unit, where a sequence has more
+ *   rows than a few tiles: 512 tokens over 4096 in 4 sequences 269 at 128, 253 at
+ *   256; 128 tokens in 4 sequences 90 and 104. Keys of fp32 fill LDS and the
+ *   registers at 128 already, so that the larger tile shares more sooner: 32
+ *   tokens over 4096 in 8 sequences 124 and 88. Heads of up to 64 are half as
+ *   much work per key, and two workgroups of 128 hide more: 8 prompts of 2502
+ *   tokens, 14 and 2 heads, 38 and 41.
+ * Pieces (target): as many as run at once, two workgroups a compute unit at
+ * 128 rows and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152 with
+ * 512); of 16 rows twice that, because sequences that decode differ in length
+ * most (64 of 1 to 8191 keys: 110 with 1024, 123 with 512), except over fp32,
+ * whose tiles leave room for one workgroup.
+ * Images: 5 us for their kernel, against splitting a key once per row tile: 1024
+ * tokens per prompt are 28 tiles (7B), where both take the same time. */
 AttnPlan plan_attention(const AttnTokens &t, int type)
 {
+    constexpr int64_t kUnits = 256;
     AttnPlan plan = {};
-    const int group = t.heads / t.kv_heads;
-    const int64_t rows = (int64_t)t.tokens * group, each = rows / t.count;
+    const int64_t heads = t.kv_heads, group = t.heads / t.kv_heads, busy = t.count < t.tokens ? t.count : t.tokens;
+    const int64_t rows = t.tokens * group, each = rows / t.count;
     const int64_t room = t.page_size ? (int64_t)t.table_stride * t.page_size : t.tokens; /* keys at most */
-    const int64_t small = (rows / 16 + (t.count < t.tokens ? t.count : t.tokens)) * t.kv_heads;
-    plan.rows = each <= 16 || (small <= 256 && small * room <= 131072) ? 16 : each <= (t.dim <= 64 ? 4096 : type == QMV_KV_F32 ? 128 : 1024) ? 128 : 256;
-#ifdef QMV_FORCE
-    plan.rows = QMV_FORCE;
-#endif
-    const int64_t tiles = rows / plan.rows + (t.count < t.tokens ? t.count : t.tokens);
+    const int64_t small = (rows / 16 + busy) * heads;
+    if (each <= 16 || (small <= kUnits && small * room <= kUnits * 512)) plan.rows = 16;
+    else if (each <= (t.dim <= 64 ? 4096 : type == QMV_KV_F32 ? 128 : 1024)) plan.rows = 128;
+    else plan.rows = 256;
+    const int64_t tiles = rows / plan.rows + busy;
     plan.tiles = (int)tiles;
-    /* As many pieces as fit the compute units at once, some more of the few-row
-     * kernel, whose sequences' lengths differ most. Prompts fill them with their
-     * tiles sooner. */
-    plan.target = plan.rows == 16 ? (type == QMV_KV_F32 ? QMV_T16F : QMV_T16) : plan.rows == 128 ? QMV_T128 : QMV_T256;
-    if (tiles * t.kv_heads >= (t.page_size ? 4096 : plan.target)) plan.target = 0;
-    plan.least = plan.rows == 16 && type != QMV_KV_F32 ? 256 : 128;
-    /* what no sequence can have more of than one piece */
-    if (room <= plan.least) plan.target = 0;
+
+    plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows == 128 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
+    plan.least = plan.rows == 16 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
+    /* None where the tiles are enough (a cache's sequences may still differ in
+     * length), or where no sequence can have more than one. */
+    if (tiles * heads >= (t.page_size ? 16 * kUnits : plan.target) || room <= plan.least) plan.target = 0;
+
     /* find_item's chunks cut all of the lengths' sum (of prompts, which attend
      * half: half of it) into max(pieces - tiles, pieces / 2), and each tile has a
      * last piece. Workgroups that find none cost their start, with the LDS of the
      * others: 8 us of 21 where there were twice as many. */
-    const int64_t pieces = plan.target / t.kv_heads;
+    const int64_t pieces = plan.target / heads;
     const int64_t items = plan.target == 0   ? tiles
                           : t.page_size == 0 ? max(2 * pieces, pieces + tiles) + 1
                                              : max(pieces, pieces / 2 + tiles) + 1;
-    plan.grid = items * t.kv_heads;
+    plan.grid = items * heads;
+    const int dp = t.dim <= 64 ? 64 : 128;
     if (plan.target) {
-        const int dp = t.dim <= 64 ? 64 : 128;
         plan.joins = (1 + (size_t)tiles) * sizeof(AttnJoin);
         plan.partials = (size_t)plan.grid * (plan.rows * (dp + 2));
     }
-    if (plan.rows == 256 && t.page_size == 0 && t.tokens / t.count >= QMV_IMG) {
-        plan.images = ((int64_t)t.tokens / kImageKeys + t.count) * t.kv_heads;
-        plan.image_bytes = (size_t)(plan.images * image_bytes(t.dim <= 64 ? 64 : 128));
+    if (plan.rows == 256 && t.page_size == 0 && t.tokens / t.count >= 1024) {
+        plan.images = ((int64_t)t.tokens / kImageKeys + t.count) * heads;
+        plan.image_bytes = (size_t)(plan.images * image_bytes(dp));
     }
     return plan;
 }
@@ -1086,7 +1094,7 @@ template <int TYPE> __global__ __launch_bounds__(256) void rope_kernel(RopeParam
     __syncthreads();
     int64_t at = -1;
     if (a.page_size && pos >= 0) {
-        at = key_at(a, s, start, pos, 0);
+        at = key_at(a, s, pos, 0);
         if (at < 0 && a.status && threadIdx.x == 0) *a.status = 0;
     }
     /* element pairs: (i, i + half) or (2 i, 2 i + 1), then what is not turned */

@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <exception>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -205,7 +206,7 @@ int workspace_reserve(Workspace &ws, hipStream_t stream, size_t bytes)
         set_error("workspace must grow during stream capture; run the call once before capturing");
         return 0;
     }
-    const size_t n = bytes + bytes / 4;
+    const size_t n = bytes + bytes / 2;
     void *buf = nullptr;
     HIP_TRY(qmv::shim_malloc(&buf, n));
     if (ws.data) ws.retired.push_back(ws.data);
@@ -215,11 +216,11 @@ int workspace_reserve(Workspace &ws, hipStream_t stream, size_t bytes)
 }
 
 int attend(qmv::AttnParams &p, int type, hipStream_t stream)
-{
+try {
     const int device = qmv::shim_device();
     HIP_TRY(hipSetDevice(device));
     const qmv::AttnPlan plan = qmv::plan_attention(p.t, type);
-    if (plan.grid > INT_MAX) {
+    if (plan.grid > INT_MAX || plan.images > INT_MAX) {
         set_error("too many tokens and heads for one call");
         return 0;
     }
@@ -234,6 +235,9 @@ int attend(qmv::AttnParams &p, int type, hipStream_t stream)
     p.joins = (qmv::AttnJoin *)(ws.data + plan.image_bytes + partial_bytes);
     HIP_TRY(qmv::launch_attention(p, plan, type, stream));
     return 1;
+} catch (const std::exception &e) { /* out of host memory */
+    set_error("%s", e.what());
+    return 0;
 }
 
 } // namespace
@@ -325,8 +329,8 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
         !row_stride_ok(d_v, &v_stride, kv_heads, head_dim, "v") ||
         !row_stride_ok(d_out, &out_stride, q_heads, head_dim, "out"))
         return 0;
-    if (!std::isfinite(scale)) {
-        set_error("scale must be finite");
+    if (!(std::fabs(scale) <= 1e38f)) { /* times log2(e) it has to be finite as well */
+        set_error("scale must be finite and at most 1e38");
         return 0;
     }
     const size_t ob = rows_bytes(tokens, out_stride, (int64_t)q_heads * head_dim);
@@ -336,16 +340,10 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
         set_error("the attention output overlaps an input");
         return 0;
     }
-    if (k_stride != v_stride) {
-        set_error("k and v must have one stride");
-        return 0;
-    }
     qmv::AttnParams p = {};
     p.t = attn_tokens(*sequences, tokens, q_heads, kv_heads, head_dim, nullptr, nullptr);
     p.t.lengths = nullptr;
     p.t.table = nullptr;
-    p.t.head_stride = head_dim;
-    p.t.token_stride = k_stride;
     p.q = d_q;
     p.k = d_k;
     p.v = d_v;
@@ -374,8 +372,8 @@ QMV_API int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride, i
     if (!row_stride_ok(d_q, &q_stride, q_heads, head_dim, "q") ||
         !row_stride_ok(d_out, &out_stride, q_heads, head_dim, "out"))
         return 0;
-    if (!std::isfinite(scale)) {
-        set_error("scale must be finite");
+    if (!(std::fabs(scale) <= 1e38f)) { /* times log2(e) it has to be finite as well */
+        set_error("scale must be finite and at most 1e38");
         return 0;
     }
     const size_t ob = rows_bytes(tokens, out_stride, (int64_t)q_heads * head_dim), cb = cache_bytes(*cache);

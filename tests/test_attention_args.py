@@ -51,7 +51,7 @@ def _rope(qmv, seq, cache, **a):
 
 SHARED = [{"tokens": 0}, {"tokens": -1}, {"tokens": (1 << 22) + 1}, {"heads": 0}, {"heads": 5}, {"heads": 65536}, {"q": None},
           {"q": BASE + 4}, {"qs": 252}, {"qs": 258}, {"qs": 1 << 31}, {"qs": -256}]
-ATTENTION = [{"scale": float("nan")}, {"scale": float("inf")}, {"out": None}, {"out": BASE + 8}, {"os": 255}, {"out": BASE},
+ATTENTION = [{"scale": float("nan")}, {"scale": float("inf")}, {"scale": -2e38}, {"out": None}, {"out": BASE + 8}, {"os": 255}, {"out": BASE},
              {"out": BASE + 1024}]
 
 

@@ -42,14 +42,15 @@ def _prompt(qmv, hip, new, heads, kv_heads, dim, q, k, v, scale, extra=(0, 0, 0)
     T = q.shape[0]
     ws, wk = heads * dim, kv_heads * dim
     qs, ks, os_ = ws + extra[0], wk + extra[1], ws + extra[2]
+    vs = wk + 2 * extra[1]
     dq = hip.DeviceBuffer.from_array(A.pack(q.reshape(T, ws), qs, ws))
-    dk, dv = (hip.DeviceBuffer.from_array(A.pack(x.reshape(T, wk), ks, wk)) for x in (k, v))
+    dk, dv = (hip.DeviceBuffer.from_array(A.pack(x.reshape(T, wk), st, wk)) for x, st in ((k, ks), (v, vs)))
     do = hip.DeviceBuffer.from_array(np.full((T, os_), MARK, np.float32))
     if starts is None:
         starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
     ds = hip.DeviceBuffer.from_array(starts)
     seq = qmv.make_sequences(ds.ptr, len(starts) - 1)
-    qmv.device_attention_prompt(dq.ptr, dk.ptr, dv.ptr, T, heads, kv_heads, dim, scale, seq, do.ptr, stream, qs, ks, ks, os_)
+    qmv.device_attention_prompt(dq.ptr, dk.ptr, dv.ptr, T, heads, kv_heads, dim, scale, seq, do.ptr, stream, qs, ks, vs, os_)
     hip.synchronize()
     out = do.to_array(np.float32, (T, os_))
     assert (out[:, ws:] == MARK).all()
@@ -81,6 +82,64 @@ def test_prompt_long(qmv, hip, n):
     o = _prompt(qmv, hip, [n], heads, kv_heads, dim, q, k, v, dim ** -0.5)
     ref, bound = A.attention64(q, k, v, dim ** -0.5, range(n))
     _check(o, ref, bound, f"prompt of {n}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,new", [
+    (4, 2, 128, [1100]),              # images of tiles, row tiles of 256
+    (2, 1, 104, [1030, 3, 1030]),     # ... of sequences that end inside a tile
+    (8, 1, 64, [1025]),               # ... of 64 elements, 8200 rows
+    (2, 2, 64, [600, 1, 0, 90]),      # row tiles of 128
+    (3, 1, 128, [100, 260]),          # row tiles of 256 without images
+])
+def test_prompt_shapes(qmv, hip, heads, kv_heads, dim, new):
+    """Each kernel that the sizes choose; only some rows are checked against 64
+    bits: the first and last of each sequence and of tiles."""
+    rng = np.random.default_rng(dim)
+    T = sum(new)
+    q, k, v = _rand(rng, T, heads, dim, wide=2), _rand(rng, T, kv_heads, dim, wide=3), _rand(rng, T, kv_heads, dim)
+    o = _prompt(qmv, hip, new, heads, kv_heads, dim, q, k, v, dim ** -0.5, extra=(4, 8, 4))
+    t = 0
+    for s, n in enumerate(new):
+        if n:
+            rows = sorted({i for i in (0, 1, 31, 32, 63, 64, 65, 127, 128, 255, 256, 257, 511, n // 2, n - 65, n - 2, n - 1)
+                           if 0 <= i < n} | set(range(0, n, 41)))
+            ref, bound = A.attention64(q[t:t + n][rows], k[t:t + n], v[t:t + n], dim ** -0.5, rows)
+            _check(o[t:t + n][rows], ref, bound, f"prompt {heads}/{kv_heads}/{dim} sequence {s} of {n}")
+        t += n
+
+
+def test_prompt_images_not_finite(qmv, hip):
+    """As test_prompt_not_finite where the keys and values are split first."""
+    rng = np.random.default_rng(8)
+    n = 1090
+    for bad in (np.inf, np.nan):
+        q, k, v = _rand(rng, n, 4, 128), _rand(rng, n, 2, 128), _rand(rng, n, 2, 128)
+        v[400, 0, 5] = v[700, 0, 5] = v[1089, 1, 100] = bad
+        k[800, 1, 3] = np.nan
+        o = _prompt(qmv, hip, [n], 4, 2, 128, q, k, v, 0.1)
+        odd = np.zeros_like(o, bool)
+        odd[400:, :2, 5] = odd[800:, 2:] = True
+        assert not np.isfinite(o[odd]).any() and np.isfinite(o[~odd]).all()
+        v[400, 0, 5] = v[700, 0, 5] = v[1089, 1, 100] = k[800, 1, 3] = 0
+        rows = [0, 399, 400, 401, 700, 799, 800, 1088, 1089]
+        ref, bound = A.attention64(q[rows], k, v, 0.1, rows)
+        keep = ~odd[rows]
+        _check(np.where(keep, o[rows], 0), np.where(keep, ref, 0), np.where(keep, bound, 1), f"images around {bad}")
+
+
+def test_prompt_many_sequences(qmv, hip):
+    """More sequences than a wave has lanes, some empty."""
+    rng = np.random.default_rng(9)
+    new = [int(x) for x in rng.integers(0, 9, 150)]
+    T = sum(new)
+    q, k, v = _rand(rng, T, 6, 64), _rand(rng, T, 2, 64), _rand(rng, T, 2, 64)
+    o = _prompt(qmv, hip, new, 6, 2, 64, q, k, v, 0.125)
+    t = 0
+    for n in new:
+        if n:
+            ref, bound = A.attention64(q[t:t + n], k[t:t + n], v[t:t + n], 0.125, range(n))
+            assert (np.abs(o[t:t + n] - ref) <= bound).all()
+        t += n
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
@@ -208,6 +267,54 @@ def test_paged_long(qmv, hip, t, new, length):
     _check_paged(b, q, keys, values, o, 128 ** -0.5, f"{A.NAMES[t]} long")
     again, _ = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
     assert np.array_equal(o.view(np.uint32), again.view(np.uint32))
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("heads,kv_heads,dim,new,length", [
+    (14, 2, 128, [190, 30], [900, 1000]),   # row tiles of 128 or 256, cut along the keys
+    (28, 1, 128, [45], [700]),              # 256 rows and more of one key head
+    (32, 1, 40, [140], [400]),              # row tiles of 256 of 64 elements
+    (8, 8, 64, [3, 20, 1], [2000, 300, 64]),
+])
+def test_paged_shapes(qmv, hip, t, heads, kv_heads, dim, new, length):
+    """Each kernel that the sizes choose; rows as in test_prompt_shapes."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, 16, seed=dim)
+    o, ok = _paged(qmv, hip, b, q, cache, dim ** -0.5)
+    assert ok == 1
+    for s, n in enumerate(new):
+        a = int(b.starts[s])
+        rows = sorted({i for i in (0, 1, 17, 18, 35, 36, 37, n - 2, n - 1) if 0 <= i < n} | set(range(0, n, 23)))
+        pos = b.positions(s)
+        ref, bound = A.attention64(q[a:a + n][rows], keys[s], values[s], dim ** -0.5, [pos[i] for i in rows])
+        _check(o[a:a + n][rows], ref, bound, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim} sequence {s} ({n} of {length[s]})")
+
+
+def test_paged_many_sequences(qmv, hip):
+    """More sequences than a wave has lanes, some idle, of very different lengths."""
+    rng = np.random.default_rng(18)
+    length = [int(x) for x in rng.integers(1, 200, 139)]
+    length[70] = 1500
+    new = [int(rng.random() < 0.8) for _ in length]
+    b, q, keys, values, cache = _paged_case(qmv, hip, new, length, 4, 2, 64, A.F16, 16, seed=19)
+    o, ok = _paged(qmv, hip, b, q, cache, 0.125)
+    assert ok == 1
+    for s, n in enumerate(new):
+        if n:
+            a = int(b.starts[s])
+            ref, bound = A.attention64(q[a:a + 1], keys[s], values[s], 0.125, [length[s] - 1])
+            assert (np.abs(o[a:a + 1] - ref) <= bound).all(), s
+
+
+def test_starts_that_fall_stay_inside(qmv, hip):
+    """Starts that do not rise: no row outside the call's is written, and the
+    call ends (every index is compared with the call's sizes)."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [10, 10, 10], [50, 60, 70], 4, 2, 64, A.F16, 16, seed=20)
+    for starts in ([0, 30, 10, 25], [-5, 100, -5, 100], [30, 20, 10, 0]):
+        b.starts = np.array(starts, np.int32)
+        o, _ = _paged(qmv, hip, b, q, cache, 0.125, 4, 4)
+        assert o.shape == q.shape
+        k = _rand(np.random.default_rng(1), 30, 2, 64)
+        _prompt(qmv, hip, None, 4, 2, 64, q, k, k, 0.125, extra=(4, 4, 4), starts=b.starts)
 
 
 def test_paged_rows_that_attend_nothing(qmv, hip):
@@ -349,6 +456,124 @@ def test_paged_graph_and_streams(qmv, hip):
                     else:
                         ref, bound = A.attention64(q[i:i + 1], keys[i], values[i], scale, [now[i] - 1])
                         _check(o[i:i + 1], ref, bound, f"replay {step} sequence {i}")
+
+
+def test_workspace(qmv, hip):
+    """A call that would have to grow its workspace in a capture is refused; a
+    graph stays right after a larger call has replaced the workspace; a size that
+    ran before allocates nothing."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, [1, 1], [700, 1300], 14, 2, 64, A.F16, 16, seed=21)
+    dq, do = hip.DeviceBuffer.from_array(q), hip.DeviceBuffer(q.nbytes)
+    seq = b.upload(qmv, hip)
+    rng = np.random.default_rng(22)
+    T = 1200
+    x = [_rand(rng, T, h, 64) for h in (14, 2, 2)]
+    dx = [hip.DeviceBuffer.from_array(a) for a in x]
+    dxo = hip.DeviceBuffer(x[0].nbytes)
+    dstarts = hip.DeviceBuffer.from_array(np.array([0, T], np.int32))
+    prompt = qmv.make_sequences(dstarts.ptr, 1)
+    far = [hip.DeviceBuffer(4 * 60000 * 256) for _ in range(4)]  # more than any test needs
+    with hip.Stream() as s:
+        with hip.Graph(s) as refused:
+            refused.begin()
+            with pytest.raises(qmv.QmvError, match="workspace"):
+                qmv.device_attention_prompt(far[0].ptr, far[1].ptr, far[2].ptr, 60000, 2, 2, 128, 0.125, prompt, far[3].ptr,
+                                            s.handle)
+            refused.end()
+        qmv.device_attention_paged(dq.ptr, 2, 14, 0.125, seq, cache.c, do.ptr, s.handle)
+        s.synchronize()
+        first = do.to_array(np.uint32, q.shape)
+        with hip.Graph(s) as g:
+            g.begin()
+            qmv.device_attention_paged(dq.ptr, 2, 14, 0.125, seq, cache.c, do.ptr, s.handle)
+            g.end()
+            for i in range(3):
+                qmv.device_attention_prompt(dx[0].ptr, dx[1].ptr, dx[2].ptr, T, 14, 2, 64, 0.125, prompt, dxo.ptr, s.handle)
+                do.fill(0xFF)
+                g.replay()
+                s.synchronize()
+                assert np.array_equal(do.to_array(np.uint32, q.shape), first), f"replay {i}"
+                count = qmv.allocation_count() if i == 0 else count
+            assert qmv.allocation_count() == count
+    ref, bound = A.attention64(x[0][::97], x[1], x[2], 0.125, list(range(T))[::97])
+    _check(dxo.to_array(np.float32, x[0].shape)[::97], ref, bound, "the larger call")
+
+
+def test_graph_of_a_step(qmv, hip):
+    """Rotary embedding, cache write and both attentions in one graph, replayed
+    with other queries and positions between eager work, against eager calls on
+    another stream with a cache of its own."""
+    rng = np.random.default_rng(23)
+    heads, kv_heads, dim, page, n = 14, 2, 64, 16, 24
+    b = A.Batch([n, 1], [n, 400], page, 6)
+    filled = [_rand(rng, m, kv_heads, dim) for m in (n + 40, 440)]
+    big = A.Batch([0, 0], [n + 40, 440], page, 6)
+    caches = [A.Cache(qmv, hip, big, filled, filled, A.BF16) for _ in range(2)]
+    b.table, b.columns = big.table, big.columns
+    seq = b.upload(qmv, hip)
+    T = b.tokens
+    d = [hip.DeviceBuffer(4 * T * w) for w in (heads * dim, kv_heads * dim, kv_heads * dim)]
+    outs = [[hip.DeviceBuffer(4 * T * w) for w in (heads * dim, kv_heads * dim, heads * dim, heads * dim)] for _ in range(2)]
+    f = hip.DeviceBuffer.from_array(A.frequencies(dim))
+
+    def step(which, stream):
+        q, k, o, p = (x.ptr for x in outs[which])
+        qmv.device_rope_append(d[0].ptr, heads, d[1].ptr, d[2].ptr, kv_heads, dim, T, f.ptr, dim, seq, q, k, caches[which].c,
+                               stream=stream.handle)
+        qmv.device_attention_paged(q, T, heads, 0.125, seq, caches[which].c, o, stream.handle)
+        qmv.device_attention_prompt(q, k, d[2].ptr, T, heads, kv_heads, dim, 0.125, seq, p, stream.handle)
+
+    with hip.Stream() as s, hip.Stream() as other:
+        step(0, s)
+        s.synchronize()
+        with hip.Graph(s) as g:
+            g.begin()
+            step(0, s)
+            g.end()
+            for i in range(4):
+                for x in d:
+                    a = rng.standard_normal(x.nbytes // 4).astype(np.float32)
+                    hip.check(hip.rt().hipMemcpy(x.ptr, a.ctypes.data, x.nbytes, hip.H2D))
+                lens = np.array([n + 10 * i, 400 + 9 * i], np.int32)
+                hip.check(hip.rt().hipMemcpy(b.d[1].ptr, lens.ctypes.data, 8, hip.H2D))
+                g.replay()
+                step(1, other)
+                s.synchronize()
+                other.synchronize()
+                for x, y in zip(*outs):
+                    assert np.array_equal(x.to_array(np.uint32, x.nbytes // 4), y.to_array(np.uint32, y.nbytes // 4)), i
+                for which in (0, 1):
+                    assert np.array_equal(caches[0].read(which), caches[1].read(which))
+
+
+def test_threads_on_their_own_streams(qmv, hip):
+    """Two host threads with a stream each, many calls at once."""
+    import threading
+    cases = [_paged_case(qmv, hip, [1, 2], [900, 500 + 300 * i], 14, 2, 64, A.F16, 16, seed=30 + i) for i in range(2)]
+    bufs = [(hip.DeviceBuffer.from_array(c[1]), hip.DeviceBuffer(c[1].nbytes), c[0].upload(qmv, hip)) for c in cases]
+    expected, failures = [], []
+    for (b, q, keys, values, cache), (dq, do, seq) in zip(cases, bufs):
+        qmv.device_attention_paged(dq.ptr, 3, 14, 0.125, seq, cache.c, do.ptr)
+        hip.synchronize()
+        expected.append(do.to_array(np.uint32, q.shape))
+
+    def work(i):
+        try:
+            (b, q, keys, values, cache), (dq, do, seq) = cases[i], bufs[i]
+            with hip.Stream() as s:
+                for _ in range(30):
+                    do.fill(0)
+                    qmv.device_attention_paged(dq.ptr, 3, 14, 0.125, seq, cache.c, do.ptr, s.handle)
+                    s.synchronize()
+                    if not np.array_equal(do.to_array(np.uint32, q.shape), expected[i]):
+                        failures.append(i)
+        except Exception as e:  # noqa: BLE001
+            failures.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert failures == []
 
 
 # ---- rotary embedding and the cache write ------------------------------------------
