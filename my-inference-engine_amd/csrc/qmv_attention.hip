@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "qmv_kernels.h"
 
 namespace qmv {
@@ -555,7 +557,8 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) {
                 int64_t from = shfl64(at, (WR == 1 ? 16 * unit_block(u) : 0) + i * PER + sub);
-                if (a.page_size == 0 && from >= 0) from = from * (unit_values(u) ? p.v_stride : p.k_stride) + kvh * dim;
+                if (a.page_size == 0 && from >= 0) /* both under 2^31 */
+                    from = (int64_t)((uint64_t)(uint32_t)from * (uint32_t)(unit_values(u) ? p.v_stride : p.k_stride)) + kvh * dim;
                 const unsigned char *src = base + (from + 8 * piece) * (TYPE == QMV_KV_F32 ? 4 : 2);
                 if (from < 0 || 8 * piece >= dim)
                     src = (const unsigned char *)(kNoPiece + (from == kNoPage && !unit_values(u) && 8 * piece < dim ? 2 : 0));
@@ -920,30 +923,35 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     float all = kNothing, sum = 0.f;
     f4_t v = {0, 0, 0, 0};
     if (real) {
-        for (int i0 = set * mine; i0 < i_end; i0 += AT_ONCE) {
-            f2_t st[AT_ONCE];
-            f4_t x[AT_ONCE];
+        /* N pieces, whose loads are in flight together */
+        auto take = [&](auto number, int i0) {
+            constexpr int N = decltype(number)::value;
+            f2_t st[N];
+            f4_t x[N];
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const float *at = from + min(i0 + i, i_end - 1) * apart;
                 st[i] = *(const f2_t *)(at + ROWS * DP + 2 * rr);
                 x[i] = *(const f4_t *)(at + rr * DP + 4 * d4);
             }
             float top = all;
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, st[i][0]);
+            for (int i = 0; i < N; ++i) top = fmaxf(top, st[i][0]);
             const float fade = __builtin_amdgcn_exp2f(all - top);
             all = top;
             sum *= fade;
             v *= fade;
 #pragma unroll
-            for (int i = 0; i < AT_ONCE; ++i)
+            for (int i = 0; i < N; ++i)
                 if (i0 + i < i_end) {
                     const float f = __builtin_amdgcn_exp2f(st[i][0] - all);
                     sum = fmaf(st[i][1], f, sum);
                     v += x[i] * f;
                 }
-        }
+        };
+        int i0 = set * mine;
+        for (; i_end - i0 > 4; i0 += AT_ONCE) take(std::integral_constant<int, AT_ONCE>(), i0);
+        if (i0 < i_end) take(std::integral_constant<int, 4>(), i0); /* the usual few without loads for nothing */
     }
     if (GROUPS > 1) {
         const int e = threadIdx.x / (D4 * GROUPS);
