@@ -448,11 +448,18 @@ int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride,
  * as it was (d_status may be null). What lies in the cache behind a sequence's
  * length is never used.
  *
- * Both forms hold q, k and v to 22 bits or more and sum in fp32. A key or value
- * that is not finite makes the rows that attend it not finite where it counts,
- * and no others. The work of few tokens is cut along the length and joined in
- * a fixed order, in a workspace of the stream, so a capture needs one call of
- * its size before it (see qmv_device_matvec_f32).
+ * Both forms multiply on the matrix cores with fp32 sums. q, the weights, and
+ * keys and values of fp32 are two f16 limbs, held to 2^-22 of themselves, or to
+ * 2^-39 of the largest of a row of q or of 16 consecutive tokens of a head,
+ * where that is more; keys and values of bf16 exactly or to that 2^-39; those
+ * of f16 exactly. Magnitudes below 2^-110 lose places. A key that is not finite
+ * makes the rows that attend it NaN, a value the elements that sum it not
+ * finite; neither reaches other rows.
+ * The work of few rows is cut along the length and joined in a fixed order: the
+ * same call gives the same bits. What the pieces pass to each other, and the
+ * limbs of long prompts, are in a workspace of the stream, so a capture needs
+ * one call of its size before it, and a graph is replayed on its stream (see
+ * qmv_device_matvec_f32).
  */
 int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride,
                                    int tokens, int q_heads, float scale,

@@ -632,6 +632,34 @@ def test_rope_append(qmv, hip, t, heads, kv_heads, dim, rotary, page, layout, in
             assert np.array_equal(after.view(np.uint8), before[which].view(np.uint8)), "codes, and all else as it was"
 
 
+def test_rows_of_one_buffer(qmv, hip):
+    """q, k and v of a token side by side in one row, turned in place, without a
+    cache, and attended from there."""
+    rng = np.random.default_rng(24)
+    heads, kv_heads, dim, T = 6, 2, 64, 90
+    wide = (heads + 2 * kv_heads) * dim
+    rows = _rand(rng, T, wide)
+    d = hip.DeviceBuffer.from_array(rows)
+    do = hip.DeviceBuffer(4 * T * heads * dim)
+    df, ds = hip.DeviceBuffer.from_array(A.frequencies(dim)), hip.DeviceBuffer.from_array(np.array([0, 30, T], np.int32))
+    seq = qmv.make_sequences(ds.ptr, 2)
+    k, v = d.ptr + 4 * heads * dim, d.ptr + 4 * (heads + kv_heads) * dim
+    qmv.device_rope_append(d.ptr, heads, k, 0, kv_heads, dim, T, df.ptr, dim, seq, d.ptr, k, q_stride=wide, k_stride=wide)
+    qmv.device_attention_prompt(d.ptr, k, v, T, heads, kv_heads, dim, 0.125, seq, do.ptr, 0, wide, wide, wide)
+    hip.synchronize()
+    turned, o = d.to_array(np.float32, rows.shape), do.to_array(np.float32, (T, heads, dim))
+    assert np.array_equal(turned[:, (heads + kv_heads) * dim:], rows[:, (heads + kv_heads) * dim:])
+    for t in range(T):
+        x = rows[t, :(heads + kv_heads) * dim].reshape(-1, dim)
+        ref = A.rope64(x, t if t < 30 else t - 30, A.frequencies(dim), False)
+        assert np.max(np.abs(turned[t, :(heads + kv_heads) * dim].reshape(-1, dim) - ref)) <= _rope_bound(x)
+    parts = turned.reshape(T, -1, dim)
+    for a, b in ((0, 30), (30, T)):
+        ref, bound = A.attention64(parts[a:b, :heads], parts[a:b, heads:heads + kv_heads], parts[a:b, heads + kv_heads:], 0.125,
+                                   range(b - a))
+        _check(o[a:b], ref, bound, f"rows {a}..{b}")
+
+
 @pytest.mark.parametrize("position", [0, 131071, 4000000, 2000000000])
 def test_rope_far_positions(qmv, hip, position):
     rng = np.random.default_rng(21)
