@@ -191,14 +191,17 @@ __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float((u
 __device__ __forceinline__ int scale_of(uint32_t bits, int most) { return min(14 - ((int)(bits >> 23) - 127), most); }
 
 /* Eight values as two limbs. In pairs, so that a limb is rounded once, packed;
- * v - hi is one instruction as a multiply-add of a half and a float. */
+ * v - hi is one instruction as a multiply-add of a half and floats, if the
+ * compiler does not know that the factor is -1. */
 __device__ __forceinline__ void limbs_of(const float *x, h8_t *hi, h8_t *lo)
 {
+    float minus;
+    asm("s_mov_b32 %0, -1.0" : "=s"(minus));
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const f2_t v = {x[i], x[i + 1]};
         const h2_t h = __builtin_convertvector(v, h2_t);
-        const f2_t rest = {fmaf((float)h[0], -1.f, v[0]), fmaf((float)h[1], -1.f, v[1])};
+        const f2_t rest = {fmaf((float)h[0], minus, v[0]), fmaf((float)h[1], minus, v[1])};
         const h2_t l = __builtin_convertvector(rest, h2_t);
         (*hi)[i] = h[0];
         (*hi)[i + 1] = h[1];
