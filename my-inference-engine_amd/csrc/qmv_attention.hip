@@ -1,7 +1,22 @@
 /*
  * gfx950 kernels between the q/k/v projections and the output projection:
- * rotary embedding with the write into a paged cache, and causal attention
- * over packed prompts and over a paged cache.
+ * rotary embedding with the write into a paged cache (rope_kernel), and causal
+ * attention over packed prompts and over a paged cache (attention_kernel, with
+ * attention_join_kernel where the keys of a row tile are cut into pieces and
+ * attention_image_kernel before long prompts).
+ *
+ * What bounds attention (28 query and 4 key heads of 128 unless said; a copy
+ * reaches 4.6 TB/s here and an 8192^3 f16 product 1.1 PFLOP/s):
+ *   one token each of 64 sequences of 1 to 8191 keys, f16 cache: the stream of
+ *   keys and values, 494 MB in 110 us with the join, 4.5 TB/s;
+ *   a prompt of 8192: the matrix cores, 1.44 T operations (three products of
+ *   limbs each) in 1.29 ms, 1.12 PFLOP/s at 2.0 GHz, where the power limit holds
+ *   the clock;
+ *   512 tokens over 16100, f16 cache: the matrix cores, 0.23 T (two products) in
+ *   251 us, 0.93 PFLOP/s with the pieces' results and their join;
+ *   small calls: their chain of memory round trips (lengths, page table, keys)
+ *   and a second launch for the join: one token over 777 keys, 14 and 2 heads of
+ *   64, 9 + 3 us.
  */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -43,7 +58,8 @@ __device__ __forceinline__ int sequence_of(const AttnTokens &a, int t)
     return a.starts[lo + 1] > t ? lo : -1;
 }
 
-/* Where key `j` of sequence s and of head h begins in a paged cache, -1 if its page is outside the cache or the table. */
+/* Where key `j` of sequence s and of head h begins in a paged cache, -1 if its
+ * page is outside the cache or the table. */
 __device__ __forceinline__ int64_t key_at(const AttnTokens &a, int s, int j, int h)
 {
     const int page = j / a.page_size;
@@ -484,8 +500,12 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
 };
 
+/* At 128 and 256 rows two waves a SIMD (except where two limbs of 128 elements
+ * and their loads do not fit 256 registers beside 128 rows: 38 would spill). At
+ * 16 rows the 4 waves have a tile each in their own LDS and need no barrier. */
 template <int TYPE, int DP, int RW, int WR, int WK>
-__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1) void attention_kernel(AttnParams p)
+__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
+void attention_kernel(AttnParams p)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
     using P = Product<RW>;
@@ -511,8 +531,6 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
     const bool found = find_item<S::ROWS, KT * WK>(p, item, lane, &it, &tiles_all);
     if (blockIdx.x == 0 && p.target && tid == 0) p.joins[0].n = tiles_all;
     if (!found) return;
-
-
     for (int i = tid; i < DP; i += THREADS) first_odd[i] = INT32_MAX;
     if (tid == 0) any_odd = 0;
     lds_barrier();
@@ -532,6 +550,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_K
     const int token = row / group, head = kvh * group + row % group;
     const bool real = token < it.n;
     const int pos = real ? it.first + token : -1;
+
     /* ---- tiles: loads into registers, then as f16 limbs into LDS ---- */
     unsigned char *tile = lds + (IMAGE ? 0 : wk * S::TILE);
     int buf = IMAGE ? 0 : wk;
@@ -1083,7 +1102,10 @@ hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type,
     return hipGetLastError();
 }
 
-/* A workgroup per token. The angle p * freq is a product in 64 bits, brought
+/* A workgroup per token: the pairs' sines once in LDS, then all heads. Bound by
+ * memory on prompts (4096 tokens, 28 and 4 heads of 128, bf16 cache: 151 MB in 27
+ * us, 5.6 TB/s), by the launch on decode steps (3 us alone, 7 for 64 tokens).
+ * The angle p * freq is a product in 64 bits, brought
  * to [-pi, pi] there: at position 10^6 an fp32 angle is off by up to 0.03.
  * What is left is rounded to fp32 once (2^-24 relative, so at most 2^-22.3
  * absolute) before the sine. */
