@@ -310,8 +310,8 @@ template <int TYPE> struct Raw {
 };
 
 /* A tile in LDS is rows of keys. Piece c of a key is at place c ^ turn(key):
- * neither the loads of one piece of many keys nor the transposing loads of a
- * few pieces of four keys meet in a bank. */
+ * neither the loads of one piece of 32 keys nor the transposing loads of a few
+ * pieces of eight meet in a bank (none counted with 32 rows a wave). */
 template <int DP> __device__ __forceinline__ int turn_of(int key)
 {
     return DP == 128 ? (key & 3) << 2 | (key >> 2 & 3) : (key >> 1 & 1) << 2 | (key >> 2 & 3);
@@ -326,6 +326,12 @@ struct AttnItem {
     int split, chunk;     /* keys [split * chunk, ...) */
 };
 
+/* What attention_list_kernel finds: pieces and row tiles of a key head, and keys
+ * of a piece at most. */
+struct AttnLists {
+    int items, tiles, chunk;
+};
+
 /* What the pieces' join has to know of a row tile whose keys are cut. */
 struct AttnJoin {
     int start, n, tile; /* as in AttnItem */
@@ -333,73 +339,115 @@ struct AttnJoin {
     int item, apart;    /* the first piece's number, and what the next ones' are apart */
 };
 
-/* The `item`-th piece of a key head's work, by one wave: of each sequence the
- * first pieces of all row tiles, the later ones (which attend more) first, then
- * their second pieces, and so on: consecutive workgroups run on different XCDs,
- * and with a tile's pieces side by side those that have no keys were all on the
- * same four (a prompt of 4096, 7B, 542 us in two pieces a tile). chunk is chosen here from all lengths, so that every workgroup
- * has the same; the sums are of floats, whose rounding the one piece beyond
- * plan_attention's count allows for. *tiles_all: row tiles in all, or 0 where
- * the starts fall so that there would be more rows than the call's. */
+/* A sequence as the kernels see it: cut to the call's tokens and its pages. */
+struct AttnSequence {
+    int start, n, len, first, tiles; /* as in AttnItem */
+};
+template <int BM> __device__ __forceinline__ AttnSequence sequence_at(const AttnTokens &a, int s)
+{
+    AttnSequence q = {};
+    if (s >= a.count) return q;
+    const int room = a.page_size ? a.table_stride * a.page_size : INT32_MAX; /* at most 2^30, or no limit */
+    q.start = min(max(a.starts[s], 0), a.tokens);
+    q.n = max(min(a.starts[s + 1], a.tokens) - q.start, 0);
+    q.len = a.lengths ? max(a.lengths[s], 0) : q.n;
+    q.first = q.len - q.n;
+    if (q.len > room) q.len = room + 1; /* one key past the table: its rows are NaN */
+    q.tiles = (q.n * (a.heads / a.kv_heads) + BM - 1) / BM;
+    return q;
+}
+
+/* What a sequence's tiles attend, or more. */
+__device__ __forceinline__ float work_of(const AttnTokens &a, const AttnSequence &q)
+{
+    return (float)q.tiles * (a.page_size ? (float)q.len : 0.5f * (float)q.len);
+}
+
+/* Keys of a piece at most, from the sums over all sequences. The sums are of
+ * floats, whose rounding the one piece beyond plan_attention's count allows
+ * for. */
+template <int STEP> __device__ __forceinline__ int chunk_of(const AttnParams &p, float work, float tiles)
+{
+    const int whole = INT32_MAX / STEP * STEP;
+    if (p.target == 0) return whole;
+    /* pieces beside the tiles' last ones, which may be short */
+    const int pieces = p.target / p.t.kv_heads;
+    const float each = work / (float)max(max(pieces - (int)tiles, pieces / 2), 1);
+    return each < 1e9f ? max(((int)each + STEP) / STEP * STEP, p.least) : whole;
+}
+
+__device__ __forceinline__ int splits_of(const AttnSequence &q, int chunk)
+{
+    return max((int)(((uint32_t)q.len + (uint32_t)chunk - 1) / (uint32_t)chunk), 1);
+}
+
+/* The `mine`-th piece of sequence s: the first pieces of all its row tiles, the
+ * later ones (which attend more) first, then their second pieces, and so on.
+ * Consecutive workgroups run on different XCDs, and with a tile's pieces side by
+ * side those that have no keys were all on the same four (a prompt of 4096, 7B,
+ * 542 us in two pieces a tile). */
+template <int STEP> __device__ __forceinline__ void piece_of(const AttnSequence &q, int s, int splits, int mine, int tiles_before, AttnItem *out)
+{
+    const int nth = mine % q.tiles;
+    out->s = s;
+    out->start = q.start;
+    out->n = q.n;
+    out->len = q.len;
+    out->first = q.first;
+    /* pieces of one length, not all but the last of a whole chunk */
+    out->chunk = ((max(q.len, 1) + splits - 1) / splits + STEP - 1) / STEP * STEP;
+    out->tiles = q.tiles;
+    out->split = mine / q.tiles;
+    out->tile = q.tiles - 1 - nth;
+    out->tile_at = tiles_before + out->tile;
+}
+
+/* The `item`-th piece of a key head's work, sequence after sequence, by one wave.
+ * Every workgroup takes the same sums over all lengths. *tiles_all: row tiles in
+ * all, or 0 where the starts fall so that there would be more rows than the
+ * call's. */
 template <int BM, int STEP>
 __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lane, AttnItem *out, int *tiles_all)
 {
     const AttnTokens &a = p.t;
-    const int group = a.heads / a.kv_heads;
-    const int room = a.page_size ? a.table_stride * a.page_size : INT32_MAX; /* at most 2^30, or no limit */
-    int start = 0, n = 0, len = 0, first = 0, tiles = 0;
-    auto read = [&](int s) {
-        start = n = len = first = tiles = 0;
-        if (s >= a.count) return;
-        start = min(max(a.starts[s], 0), a.tokens);
-        n = max(min(a.starts[s + 1], a.tokens) - start, 0);
-        len = a.lengths ? max(a.lengths[s], 0) : n;
-        first = len - n;
-        if (len > room) len = room + 1; /* one key past the table: its rows are NaN */
-        tiles = (n * group + BM - 1) / BM;
-    };
-    float work = 0.f, rows = 0.f, tiles_sum = 0.f;
+    if (p.lists) { /* attention_list_kernel has looked already */
+        const AttnLists &lists = *p.lists;
+        *tiles_all = lists.tiles;
+        if (item >= lists.items) return false;
+        const int s = __builtin_amdgcn_readfirstlane(p.sequence_of_item[item]);
+        const AttnSequence q = sequence_at<BM>(a, s);
+        const int2 before = p.before[s];
+        piece_of<STEP>(q, s, splits_of(q, lists.chunk), item - before.x, before.y, out);
+        return true;
+    }
+    AttnSequence q;
+    float work = 0.f, rows = 0.f, tiles = 0.f;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
-        read(s0 + lane);
-        work += (float)tiles * (a.page_size ? (float)len : 0.5f * (float)len); /* what the tiles attend, or more */
-        rows += (float)n;
-        tiles_sum += (float)tiles;
+        q = sequence_at<BM>(a, s0 + lane);
+        work += work_of(a, q);
+        rows += (float)q.n;
+        tiles += (float)q.tiles;
     }
     work = lane_of(scan_lanes(work), 63);
     rows = lane_of(scan_lanes(rows), 63);
-    tiles_sum = lane_of(scan_lanes(tiles_sum), 63);
+    tiles = lane_of(scan_lanes(tiles), 63);
     *tiles_all = 0;
     if (rows > (float)a.tokens) return false;
-    int chunk = INT32_MAX / STEP * STEP;
-    if (p.target) {
-        /* pieces beside the tiles' last ones, which may be short */
-        const int pieces = p.target / a.kv_heads, tiles_in_all = (int)tiles_sum;
-        const float each = work / (float)max(max(pieces - tiles_in_all, pieces / 2), 1);
-        chunk = each < 1e9f ? max(((int)each + STEP) / STEP * STEP, p.least) : chunk;
-    }
+    const int chunk = chunk_of<STEP>(p, work, tiles);
     int before = 0, tiles_before = 0;
     bool found = false;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
-        if (a.count > 64) read(s0 + lane);
-        const int splits = max((int)(((uint32_t)len + (uint32_t)chunk - 1) / (uint32_t)chunk), 1);
-        const int items = tiles * splits;
-        const int sum = scan_lanes(items), tsum = scan_lanes(tiles);
+        if (a.count > 64) q = sequence_at<BM>(a, s0 + lane);
+        const int splits = splits_of(q, chunk);
+        const int items = q.tiles * splits;
+        const int sum = scan_lanes(items), tsum = scan_lanes(q.tiles);
         const uint64_t hit = __ballot(before + sum > item);
         if (hit && !found) {
             const int at = __builtin_ctzll(hit);
-            const int mine = item - before - (lane_of(sum, at) - lane_of(items, at));
-            const int sp = lane_of(splits, at), all = lane_of(tiles, at), nth = mine % all;
-            out->s = s0 + at;
-            out->start = lane_of(start, at);
-            out->n = lane_of(n, at);
-            out->len = lane_of(len, at);
-            out->first = lane_of(first, at);
-            /* pieces of one length, not all but the last of `chunk` */
-            out->chunk = ((max(out->len, 1) + sp - 1) / sp + STEP - 1) / STEP * STEP;
-            out->tiles = all;
-            out->split = mine / all;
-            out->tile = all - 1 - nth;
-            out->tile_at = tiles_before + lane_of(tsum, at) - all + out->tile;
+            const AttnSequence mine = {lane_of(q.start, at), lane_of(q.n, at), lane_of(q.len, at), lane_of(q.first, at),
+                                       lane_of(q.tiles, at)};
+            piece_of<STEP>(mine, s0 + at, lane_of(splits, at), item - before - (lane_of(sum, at) - lane_of(items, at)),
+                           tiles_before + lane_of(tsum, at) - mine.tiles, out);
             found = true;
         }
         before += lane_of(sum, 63);
@@ -408,6 +456,79 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     }
     *tiles_all = tiles_before;
     return found;
+}
+
+/* Many sequences: what find_item would look for in every workgroup, once. One
+ * workgroup: the sums and the chunk, then 1024 sequences at a time the items
+ * and tiles before each and each item's sequence. (8192 sequences of 200 keys,
+ * 28 and 4 heads: 9.7 ms without.) */
+template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_list_kernel(AttnParams p)
+{
+    __shared__ float sums[3][16];
+    __shared__ int ends[1024], tile_ends[16], item_ends[16];
+    const AttnTokens &a = p.t;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float work = 0.f, rows = 0.f, tiles = 0.f;
+    for (int s = tid; s < a.count; s += 1024) {
+        const AttnSequence q = sequence_at<BM>(a, s);
+        work += work_of(a, q);
+        rows += (float)q.n;
+        tiles += (float)q.tiles;
+    }
+    work = scan_lanes(work);
+    rows = scan_lanes(rows);
+    tiles = scan_lanes(tiles);
+    if (lane == 63) {
+        sums[0][wave] = work;
+        sums[1][wave] = rows;
+        sums[2][wave] = tiles;
+    }
+    __syncthreads();
+    work = rows = tiles = 0.f;
+    for (int i = 0; i < 16; ++i) {
+        work += sums[0][i];
+        rows += sums[1][i];
+        tiles += sums[2][i];
+    }
+    const int chunk = chunk_of<STEP>(p, work, tiles);
+    const bool valid = rows <= (float)a.tokens;
+    int items_before = 0, tiles_before = 0;
+    for (int s0 = 0; valid && s0 < a.count; s0 += 1024) {
+        const AttnSequence q = sequence_at<BM>(a, s0 + tid);
+        const int items = q.tiles * splits_of(q, chunk);
+        int sum = scan_lanes(items), tsum = scan_lanes(q.tiles);
+        if (lane == 63) {
+            item_ends[wave] = sum;
+            tile_ends[wave] = tsum;
+        }
+        __syncthreads();
+        int all = 0, tall = 0;
+        for (int i = 0; i < 16; ++i) {
+            if (i < wave) {
+                sum += item_ends[i];
+                tsum += tile_ends[i];
+            }
+            all += item_ends[i];
+            tall += tile_ends[i];
+        }
+        ends[tid] = sum;
+        if (s0 + tid < a.count) p.before[s0 + tid] = int2{items_before + sum - items, tiles_before + tsum - q.tiles};
+        __syncthreads();
+        for (int i = tid; i < all; i += 1024) {
+            if (items_before + i >= p.most_items) break;
+            int lo = 0, hi = 1023; /* the first sequence whose items end past i */
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ends[mid] > i) hi = mid;
+                else lo = mid + 1;
+            }
+            p.sequence_of_item[items_before + i] = s0 + lo;
+        }
+        items_before += all;
+        tiles_before += tall;
+        __syncthreads();
+    }
+    if (tid == 0) *p.lists = AttnLists{min(items_before, p.most_items), tiles_before, chunk};
 }
 
 /* Long prompts: their keys and values are split into limbs once, as images of
@@ -1050,6 +1171,10 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
                           : t.page_size == 0 ? max(2 * pieces, pieces + tiles) + 1
                                              : max(pieces, pieces / 2 + tiles) + 1;
     plan.grid = items * heads;
+    plan.items = (int)items;
+    /* A list where every workgroup would read more than 256 sequences' lengths: 512
+     * of 1000 keys 243 us without, 2048 of 500 854. */
+    if (t.count > 256) plan.lists = sizeof(AttnLists) + (size_t)t.count * sizeof(int2) + (size_t)items * sizeof(int) + 16;
     const int dp = t.dim <= 64 ? 64 : 128;
     if (plan.target) {
         plan.joins = (1 + (size_t)tiles) * sizeof(AttnJoin);
@@ -1064,6 +1189,8 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
 
 template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
+    using S = AttnShape<TYPE, DP, RW, WR, WK>;
+    if (plan.lists) attention_list_kernel<S::ROWS, S::KT * WK><<<1, 1024, 0, s>>>(p);
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
     constexpr int ROWS = RW * WR, GROUPS = ROWS == 16 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);

@@ -187,12 +187,15 @@ struct Workspace {
 };
 
 std::mutex g_workspaces_mu;
-std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>> g_workspaces;
+std::map<std::pair<int, const void *>, std::unique_ptr<Workspace>> g_workspaces;
+
+/* Threads share the handle of the per-thread stream and not the stream. */
+thread_local char t_stream;
 
 Workspace &workspace_for(int device, hipStream_t stream)
 {
     std::lock_guard<std::mutex> lock(g_workspaces_mu);
-    auto &slot = g_workspaces[{device, stream}];
+    auto &slot = g_workspaces[{device, stream == hipStreamPerThread ? (const void *)&t_stream : (const void *)stream}];
     if (!slot) slot.reset(new Workspace());
     return *slot;
 }
@@ -226,13 +229,22 @@ try {
     }
     Workspace &ws = workspace_for(device, stream);
     std::lock_guard<std::mutex> lock(ws.mu);
-    const size_t partial_bytes = plan.partials * sizeof(float);
-    if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + plan.joins)) return 0;
+    const size_t partial_bytes = plan.partials * sizeof(float), joins = (plan.joins + 15) / 16 * 16;
+    const size_t counts = (size_t)p.t.count * sizeof(int2);
+    if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + joins + plan.lists)) return 0;
+    unsigned char *at = ws.data;
     p.target = plan.target;
     p.least = plan.least;
-    p.image = ws.data;
-    p.partials = (float *)(ws.data + plan.image_bytes);
-    p.joins = (qmv::AttnJoin *)(ws.data + plan.image_bytes + partial_bytes);
+    p.image = at;
+    p.partials = (float *)(at += plan.image_bytes);
+    p.joins = (qmv::AttnJoin *)(at += partial_bytes);
+    at += joins;
+    if (plan.lists) { /* the head takes 16 bytes */
+        p.lists = (qmv::AttnLists *)at;
+        p.before = (int2 *)(at + 16);
+        p.sequence_of_item = (int *)(at + 16 + counts);
+        p.most_items = plan.items;
+    }
     HIP_TRY(qmv::launch_attention(p, plan, type, stream));
     return 1;
 } catch (const std::exception &e) { /* out of host memory */

@@ -162,6 +162,7 @@ struct AttnTokens {
 };
 
 struct AttnJoin;
+struct AttnLists;
 struct AttnParams {
     AttnTokens t;
     const float *q;
@@ -177,6 +178,12 @@ struct AttnParams {
     float *partials;
     unsigned char *image; /* a prompt's keys and values as tiles of limbs */
     AttnJoin *joins; /* [0].n: row tiles in all; [1 + tile] */
+    /* Of many sequences (null otherwise): the list's head, the items and tiles
+     * before each sequence, and each item's sequence (most_items of them). */
+    AttnLists *lists;
+    int2 *before;
+    int *sequence_of_item;
+    int most_items;
 };
 
 /* How a call is launched: rows (token, head of the group) per workgroup, the
@@ -186,7 +193,9 @@ struct AttnPlan {
     int target, least;
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
+    int items;              /* pieces at most, of one key head */
     size_t partials, joins; /* floats, bytes */
+    size_t lists;           /* bytes, 0: none */
     int64_t images;         /* tiles that are made first, 0: none */
     size_t image_bytes;
 };

@@ -127,10 +127,11 @@ def test_prompt_images_not_finite(qmv, hip):
         _check(np.where(keep, o[rows], 0), np.where(keep, ref, 0), np.where(keep, bound, 1), f"images around {bad}")
 
 
-def test_prompt_many_sequences(qmv, hip):
-    """More sequences than a wave has lanes, some empty."""
+@pytest.mark.parametrize("count,longest", [(150, 9), (400, 9), (300, 60)])
+def test_prompt_many_sequences(qmv, hip, count, longest):
+    """As test_paged_many_sequences, some empty."""
     rng = np.random.default_rng(9)
-    new = [int(x) for x in rng.integers(0, 9, 150)]
+    new = [int(x) for x in rng.integers(0, longest, count)]
     T = sum(new)
     q, k, v = _rand(rng, T, 6, 64), _rand(rng, T, 2, 64), _rand(rng, T, 2, 64)
     o = _prompt(qmv, hip, new, 6, 2, 64, q, k, v, 0.125)
@@ -289,10 +290,12 @@ def test_paged_shapes(qmv, hip, t, heads, kv_heads, dim, new, length):
         _check(o[a:a + n][rows], ref, bound, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim} sequence {s} ({n} of {length[s]})")
 
 
-def test_paged_many_sequences(qmv, hip):
-    """More sequences than a wave has lanes, some idle, of very different lengths."""
+@pytest.mark.parametrize("count,longest", [(139, 200), (257, 40), (2500, 30)])
+def test_paged_many_sequences(qmv, hip, count, longest):
+    """More sequences than a wave has lanes, or than workgroups look through
+    themselves; some idle, one far longer."""
     rng = np.random.default_rng(18)
-    length = [int(x) for x in rng.integers(1, 200, 139)]
+    length = [int(x) for x in rng.integers(1, longest, count)]
     length[70] = 1500
     new = [int(rng.random() < 0.8) for _ in length]
     b, q, keys, values, cache = _paged_case(qmv, hip, new, length, 4, 2, 64, A.F16, 16, seed=19)
@@ -309,8 +312,12 @@ def test_starts_that_fall_stay_inside(qmv, hip):
     """Starts that do not rise: no row outside the call's is written, and the
     call ends (every index is compared with the call's sizes)."""
     b, q, keys, values, cache = _paged_case(qmv, hip, [10, 10, 10], [50, 60, 70], 4, 2, 64, A.F16, 16, seed=20)
-    for starts in ([0, 30, 10, 25], [-5, 100, -5, 100], [30, 20, 10, 0]):
+    table, length = b.table, b.length
+    falling = [int(x) for x in np.random.default_rng(2).integers(-9, 40, 301)]
+    for starts in ([0, 30, 10, 25], [-5, 100, -5, 100], [30, 20, 10, 0], falling):
         b.starts = np.array(starts, np.int32)
+        times = -(-(len(starts) - 1) // 3)
+        b.new, b.length, b.table = [0] * (len(starts) - 1), (length * times)[:len(starts) - 1], np.concatenate([table] * times)
         o, _ = _paged(qmv, hip, b, q, cache, 0.125, 4, 4)
         assert o.shape == q.shape
         k = _rand(np.random.default_rng(1), 30, 2, 64)
