@@ -1043,7 +1043,7 @@ void attention_kernel(AttnParams p)
  * joined by the last workgroup of a tile, the 128 pieces of one row tile at
  * 32749 keys took 17 us of one compute unit. */
 template <int DP, int ROWS, int GROUPS>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float down)
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int slices, float down)
 {
     constexpr int D4 = DP / 4, EACH = 256 / (D4 * GROUPS); /* rows of a workgroup */
     constexpr int AT_ONCE = GROUPS > 1 ? 8 : 16;
@@ -1051,72 +1051,73 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, float
     __shared__ f4_t sums[GROUPS > 1 ? GROUPS : 1][EACH][D4];
     __shared__ f2_t states[GROUPS > 1 ? GROUPS : 1][EACH];
     const AttnTokens &a = p.t;
-    const int slices = ROWS / EACH, group = a.heads / a.kv_heads;
+    const int group = a.heads / a.kv_heads;
     const int slice = blockIdx.x % slices, rest = blockIdx.x / slices, kvh = rest % a.kv_heads, tile_at = rest / a.kv_heads;
     const int tiles = p.joins[0].n;
     const AttnJoin j = p.joins[1 + tile_at]; /* of no meaning past `tiles` */
     if (tile_at >= tiles || j.pieces == 0) return;
-    const int d4 = threadIdx.x % D4, set = threadIdx.x / D4 % GROUPS, rr = slice * EACH + threadIdx.x / (D4 * GROUPS);
-    const int row = j.tile * ROWS + rr, token = row / group;
-    if (j.tile * ROWS + slice * EACH >= j.n * group) return; /* no row of this workgroup */
-    const bool real = token < j.n;
+    const int d4 = threadIdx.x % D4, set = threadIdx.x / D4 % GROUPS, each = threadIdx.x / (D4 * GROUPS);
     const float *from = p.partials + ((int64_t)j.item * a.kv_heads + kvh) * PARTIAL;
     const int64_t apart = (int64_t)j.apart * a.kv_heads * PARTIAL;
     const int mine = (j.pieces + GROUPS - 1) / GROUPS, i_end = min((set + 1) * mine, j.pieces);
-    float all = kNothing, sum = 0.f;
-    f4_t v = {0, 0, 0, 0};
-    if (real) {
-        /* N pieces, whose loads are in flight together */
-        auto take = [&](auto number, int i0) {
-            constexpr int N = decltype(number)::value;
-            f2_t st[N];
-            f4_t x[N];
+    const int rows = min(ROWS, j.n * group - j.tile * ROWS);
+    for (int r0 = slice * EACH; r0 < rows; r0 += slices * EACH) {
+        const int rr = r0 + each, row = j.tile * ROWS + rr, token = row / group;
+        const bool real = rr < rows;
+        float all = kNothing, sum = 0.f;
+        f4_t v = {0, 0, 0, 0};
+        if (real) {
+            /* N pieces, whose loads are in flight together */
+            auto take = [&](auto number, int i0) {
+                constexpr int N = decltype(number)::value;
+                f2_t st[N];
+                f4_t x[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float *at = from + min(i0 + i, i_end - 1) * apart;
-                st[i] = *(const f2_t *)(at + ROWS * DP + 2 * rr);
-                x[i] = *(const f4_t *)(at + rr * DP + 4 * d4);
-            }
-            float top = all;
-#pragma unroll
-            for (int i = 0; i < N; ++i) top = fmaxf(top, st[i][0]);
-            const float fade = __builtin_amdgcn_exp2f(all - top);
-            all = top;
-            sum *= fade;
-            v *= fade;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i0 + i < i_end) {
-                    const float f = __builtin_amdgcn_exp2f(st[i][0] - all);
-                    sum = fmaf(st[i][1], f, sum);
-                    v += x[i] * f;
+                for (int i = 0; i < N; ++i) {
+                    const float *at = from + min(i0 + i, i_end - 1) * apart;
+                    st[i] = *(const f2_t *)(at + ROWS * DP + 2 * rr);
+                    x[i] = *(const f4_t *)(at + rr * DP + 4 * d4);
                 }
-        };
-        int i0 = set * mine;
-        for (; i_end - i0 > 4; i0 += AT_ONCE) take(std::integral_constant<int, AT_ONCE>(), i0);
-        if (i0 < i_end) take(std::integral_constant<int, 4>(), i0); /* the usual few without loads for nothing */
-    }
-    if (GROUPS > 1) {
-        const int e = threadIdx.x / (D4 * GROUPS);
-        sums[set][e][d4] = v;
-        if (d4 == 0) states[set][e] = f2_t{all, sum};
-        __syncthreads();
-        if (set > 0) return;
-        float top = all;
+                float top = all;
 #pragma unroll
-        for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, states[i][e][0]);
-        v = f4_t{0, 0, 0, 0};
-        sum = 0.f;
+                for (int i = 0; i < N; ++i) top = fmaxf(top, st[i][0]);
+                const float fade = __builtin_amdgcn_exp2f(all - top);
+                all = top;
+                sum *= fade;
+                v *= fade;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            const float f = __builtin_amdgcn_exp2f(states[i][e][0] - top);
-            sum = fmaf(states[i][e][1], f, sum);
-            v += sums[i][e][d4] * f;
+                for (int i = 0; i < N; ++i)
+                    if (i0 + i < i_end) {
+                        const float f = __builtin_amdgcn_exp2f(st[i][0] - all);
+                        sum = fmaf(st[i][1], f, sum);
+                        v += x[i] * f;
+                    }
+            };
+            int i0 = set * mine;
+            for (; i_end - i0 > 4; i0 += AT_ONCE) take(std::integral_constant<int, AT_ONCE>(), i0);
+            if (i0 < i_end) take(std::integral_constant<int, 4>(), i0); /* the usual few without loads for nothing */
         }
-    }
-    if (real && 4 * d4 < a.dim) {
-        float *out = p.out + (int64_t)(j.start + token) * p.out_stride + (int64_t)(kvh * group + row - token * group) * a.dim;
-        *(f4_t *)(out + 4 * d4) = v * (sum == 0.f ? 0.f : down / sum);
+        if (GROUPS > 1) {
+            sums[set][each][d4] = v;
+            if (d4 == 0) states[set][each] = f2_t{all, sum};
+            __syncthreads();
+            float top = states[0][each][0];
+#pragma unroll
+            for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, states[i][each][0]);
+            v = f4_t{0, 0, 0, 0};
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const float f = __builtin_amdgcn_exp2f(states[i][each][0] - top);
+                sum = fmaf(states[i][each][1], f, sum);
+                v += sums[i][each][d4] * f;
+            }
+            __syncthreads();
+        }
+        if (real && set == 0 && 4 * d4 < a.dim) {
+            float *out = p.out + (int64_t)(j.start + token) * p.out_stride + (int64_t)(kvh * group + row - token * group) * a.dim;
+            *(f4_t *)(out + 4 * d4) = v * (sum == 0.f ? 0.f : down / sum);
+        }
     }
 }
 
@@ -1194,8 +1195,11 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
     constexpr int ROWS = RW * WR, GROUPS = ROWS == 16 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
-    const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * (ROWS / EACH));
-    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
+    /* of a tile of 16, workgroups for the rows that a sequence has on average */
+    const int64_t each = ((int64_t)p.t.tokens * (p.t.heads / p.t.kv_heads) + p.t.count - 1) / p.t.count;
+    const int slices = (int)(((ROWS == 16 && each < ROWS ? each : ROWS) + EACH - 1) / EACH);
+    const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * slices);
+    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
 }
 
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
