@@ -363,15 +363,34 @@ __device__ __forceinline__ float work_of(const AttnTokens &a, const AttnSequence
     return (float)q.tiles * (a.page_size ? (float)q.len : 0.5f * (float)q.len);
 }
 
-/* Keys of a piece at most, from the sums over all sequences. The sums are of
- * floats, whose rounding the one piece beyond plan_attention's count allows
- * for. */
-template <int STEP> __device__ __forceinline__ int chunk_of(const AttnParams &p, float work, float tiles)
+/* Keys of a piece at most, from the sums over all sequences and the longest
+ * that brings tokens; a whole wave asks. The sums are of floats, whose rounding
+ * the one piece beyond plan_attention's count allows for.
+ *
+ * Where the lengths are alike (and slots is set: 16 rows over f16 or bf16) each
+ * lane takes a number of pieces per tile and says what it costs: rounds of the
+ * workgroups that run at once, each as long as its keys and 64 more for its
+ * start, less where a single round leaves compute units to one workgroup, which
+ * streams up to 1 / 0.58 times as fast as two. 28 and 4 heads of 128, f16, with
+ * and without (us): 64 sequences of 1000 keys 33 / 42, of 4000 108 / 121, 16 of
+ * 4000 33 / 41. */
+template <int STEP> __device__ __forceinline__ int chunk_of(const AttnParams &p, float work, float tiles, int longest)
 {
     const int whole = INT32_MAX / STEP * STEP;
     if (p.target == 0) return whole;
-    /* pieces beside the tiles' last ones, which may be short */
     const int pieces = p.target / p.t.kv_heads;
+    if (p.slots && tiles * (float)longest <= 1.1f * work && tiles * 64.f >= (float)pieces) {
+        const int lane = threadIdx.x & 63, n = lane + 1;
+        const int keys = max((longest / n + STEP) / STEP * STEP, STEP); /* n of them reach `longest` */
+        const float items = tiles * (float)n, load = items * (float)p.t.kv_heads / (float)p.slots;
+        const float cost = (float)(keys + 64) * (load > 1.f ? ceilf(load) : fmaxf(load, 0.58f));
+        const bool fits = lane == 0 || (items <= (float)pieces && keys >= p.least);
+        /* the cheapest, of the same cost the fewest pieces */
+        const uint32_t worth = fits ? ~(__float_as_uint(cost) & ~63u | (uint32_t)lane) : 0u;
+        const int best = (int)(~wave_max(worth) & 63u);
+        return lane_of(keys, best);
+    }
+    /* pieces beside the tiles' last ones, which may be short */
     const float each = work / (float)max(max(pieces - (int)tiles, pieces / 2), 1);
     return each < 1e9f ? max(((int)each + STEP) / STEP * STEP, p.least) : whole;
 }
@@ -422,8 +441,10 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     }
     AttnSequence q;
     float work = 0.f, rows = 0.f, tiles = 0.f;
+    int longest = 0;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         q = sequence_at<BM>(a, s0 + lane);
+        longest = max(longest, q.n > 0 ? q.len : 0);
         work += work_of(a, q);
         rows += (float)q.n;
         tiles += (float)q.tiles;
@@ -433,7 +454,7 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     tiles = lane_of(scan_lanes(tiles), 63);
     *tiles_all = 0;
     if (rows > (float)a.tokens) return false;
-    const int chunk = chunk_of<STEP>(p, work, tiles);
+    const int chunk = chunk_of<STEP>(p, work, tiles, (int)wave_max((uint32_t)longest));
     int before = 0, tiles_before = 0;
     bool found = false;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
@@ -465,12 +486,14 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
 template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_list_kernel(AttnParams p)
 {
     __shared__ float sums[3][16];
-    __shared__ int ends[1024], tile_ends[16], item_ends[16];
+    __shared__ int longests[16], ends[1024], tile_ends[16], item_ends[16];
     const AttnTokens &a = p.t;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float work = 0.f, rows = 0.f, tiles = 0.f;
+    int longest = 0;
     for (int s = tid; s < a.count; s += 1024) {
         const AttnSequence q = sequence_at<BM>(a, s);
+        longest = max(longest, q.n > 0 ? q.len : 0);
         work += work_of(a, q);
         rows += (float)q.n;
         tiles += (float)q.tiles;
@@ -478,7 +501,9 @@ template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_li
     work = scan_lanes(work);
     rows = scan_lanes(rows);
     tiles = scan_lanes(tiles);
+    longest = (int)wave_max((uint32_t)longest);
     if (lane == 63) {
+        longests[wave] = longest;
         sums[0][wave] = work;
         sums[1][wave] = rows;
         sums[2][wave] = tiles;
@@ -489,8 +514,9 @@ template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_li
         work += sums[0][i];
         rows += sums[1][i];
         tiles += sums[2][i];
+        longest = max(longest, longests[i]);
     }
-    const int chunk = chunk_of<STEP>(p, work, tiles);
+    const int chunk = chunk_of<STEP>(p, work, tiles, longest);
     const bool valid = rows <= (float)a.tokens;
     int items_before = 0, tiles_before = 0;
     for (int s0 = 0; valid && s0 < a.count; s0 += 1024) {
@@ -1158,6 +1184,7 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     plan.tiles = (int)tiles;
 
     plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows == 128 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
+    plan.slots = plan.rows == 16 && t.page_size && type != QMV_KV_F32 ? (int)(2 * kUnits) : 0;
     plan.least = plan.rows == 16 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
     /* None where the tiles are enough (a cache's sequences may still differ in
      * length), or where no sequence can have more than one. */

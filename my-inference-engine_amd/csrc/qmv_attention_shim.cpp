@@ -235,6 +235,7 @@ try {
     unsigned char *at = ws.data;
     p.target = plan.target;
     p.least = plan.least;
+    p.slots = plan.slots;
     p.image = at;
     p.partials = (float *)(at += plan.image_bytes);
     p.joins = (qmv::AttnJoin *)(at += partial_bytes);

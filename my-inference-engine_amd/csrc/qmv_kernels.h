@@ -175,6 +175,7 @@ struct AttnParams {
      * not), whose partial results meet in the workspace. */
     int target;
     int least; /* keys of a piece at least, whole steps of the kernel */
+    int slots; /* workgroups that run at once, 0: the pieces are not fitted to them */
     float *partials;
     unsigned char *image; /* a prompt's keys and values as tiles of limbs */
     AttnJoin *joins; /* [0].n: row tiles in all; [1 + tile] */
@@ -190,7 +191,7 @@ struct AttnParams {
  * workgroups and the workspace. */
 struct AttnPlan {
     int rows;
-    int target, least;
+    int target, least, slots;
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
     int items;              /* pieces at most, of one key head */
