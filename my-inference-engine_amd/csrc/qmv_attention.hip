@@ -367,7 +367,7 @@ __device__ __forceinline__ float work_of(const AttnTokens &a, const AttnSequence
  * that brings tokens; a whole wave asks. The sums are of floats, whose rounding
  * the one piece beyond plan_attention's count allows for.
  *
- * Where the lengths are alike (and slots is set: 16 rows over f16 or bf16) each
+ * Where the lengths are alike (and slots is set: up to 32 rows over f16 or bf16) each
  * lane takes a number of pieces per tile and says what it costs: rounds of the
  * workgroups that run at once, each as long as its keys and 64 more for its
  * start, less where a single round leaves compute units to one workgroup, which
@@ -647,11 +647,13 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
 };
 
-/* At 128 and 256 rows two waves a SIMD (except where two limbs of 128 elements
- * and their loads do not fit 256 registers beside 128 rows: 38 would spill). At
- * 16 rows the 4 waves have a tile each in their own LDS and need no barrier. */
+/* From 32 rows on two waves a SIMD (except where two limbs of 128 elements and
+ * their loads do not fit 256 registers beside 32 rows of a wave: 38 would spill;
+ * with one, of f16 keys, 32 rows take 149 us for 4 tokens each over 64 sequences
+ * of 4000, and 112 with two). At 16 and 32 rows the 4 waves have a tile each in
+ * their own LDS and need no barrier. */
 template <int TYPE, int DP, int RW, int WR, int WK>
-__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (WR == 4 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
+__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (RW == 32 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
 void attention_kernel(AttnParams p)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
@@ -697,6 +699,9 @@ void attention_kernel(AttnParams p)
     const int token = row / group, head = kvh * group + row % group;
     const bool real = token < it.n;
     const int pos = real ? it.first + token : -1;
+    /* A wave without rows only loads: 24 of 128 rows over 4000 keys 179 us
+     * otherwise, 169 so. */
+    const bool works = WR == 1 || it.tile * S::ROWS + wr * RW < it.n * group;
 
     /* ---- tiles: loads into registers, then as f16 limbs into LDS ---- */
     unsigned char *tile = lds + (IMAGE ? 0 : wk * S::TILE);
@@ -969,7 +974,7 @@ void attention_kernel(AttnParams p)
                     if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) atomicMin(&first_odd[d], j);
                 }
             }
-            compute(k0);
+            if (works) compute(k0);
             buf ^= 1;
             tile = lds + buf * S::TILE;
         }
@@ -982,7 +987,7 @@ void attention_kernel(AttnParams p)
             next = place(k0 + 2 * STEP);
             if (WR > 1) lds_barrier();
             else asm volatile("" ::: "memory");
-            if (k0 < end) compute(k0);
+            if (k0 < end && works) compute(k0);
             if (WR == 1) asm volatile("" ::: "memory");
         }
     }
@@ -1160,8 +1165,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
  *   the 256 compute units and the keys are few enough that reading them for
  *   each tile costs less than the larger tiles' start: prompt of 37 tokens 10.9 /
  *   13.2 / 16.4, of 128 11.5 / 18.4 / 21.7, of 256 28.8 / 25.4 / 28.9; 32 tokens
- *   over 512 15.7 / 19.1 / 22.4, over 4096 32.8 / 28.0 / 30.2. (32 rows, tried,
- *   were slower than 16 or than 128 at every size.)
+ *   over 512 15.7 / 19.1 / 22.4, over 4096 32.8 / 28.0 / 30.2.
+ *   32, over a cache, where sequences have 17 to 32 rows, a few tokens that are
+ *   checked at once: 4 tokens over 4000 keys in 64 sequences 180 / (32 rows) 113 /
+ *   (128 rows) 214, over 500 in 256 148 / 88 / 99; of fp32 420 / 242 / 380. Two
+ *   tiles of 32 read keys twice: 8 tokens over 16000 in 16 sequences 238, 165 at
+ *   128. Prompts of 24 rows do better at 128 (64 of them 21 and 17).
  *   256, one workgroup of 8 waves per compute unit, where a sequence has more
  *   rows than a few tiles: 512 tokens over 4096 in 4 sequences 269 at 128, 253 at
  *   256; 128 tokens in 4 sequences 90 and 104. Keys of fp32 fill LDS and the
@@ -1170,7 +1179,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
  *   much work per key, and two workgroups of 128 hide more: 8 prompts of 2502
  *   tokens, 14 and 2 heads, 38 and 41.
  * Pieces (target): as many as run at once, two workgroups a compute unit at
- * 128 rows and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152 with
+ * 32 and 128 rows and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152 with
  * 512); of 16 rows twice that, because sequences that decode differ in length
  * most (64 of 1 to 8191 keys: 110 with 1024, 123 with 512), except over fp32,
  * whose tiles leave room for one workgroup.
@@ -1185,14 +1194,15 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     const int64_t room = t.page_size ? (int64_t)t.table_stride * t.page_size : t.tokens; /* keys at most */
     const int64_t small = (rows / 16 + busy) * heads;
     if (each <= 16 || (small <= kUnits && small * room <= kUnits * 512)) plan.rows = 16;
+    else if (each <= 32 && t.page_size) plan.rows = 32;
     else if (each <= (t.dim <= 64 ? 4096 : type == QMV_KV_F32 ? 128 : 1024)) plan.rows = 128;
     else plan.rows = 256;
     const int64_t tiles = rows / plan.rows + busy;
     plan.tiles = (int)tiles;
 
-    plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows == 128 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
-    plan.slots = plan.rows == 16 && t.page_size && type != QMV_KV_F32 ? (int)(2 * kUnits) : 0;
-    plan.least = plan.rows == 16 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
+    plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows != 16 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
+    plan.slots = plan.rows <= 32 && t.page_size && type != QMV_KV_F32 ? (int)(2 * kUnits) : 0;
+    plan.least = plan.rows <= 32 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
     /* None where the tiles are enough (a cache's sequences may still differ in
      * length), or where no sequence can have more than one. */
     if (tiles * heads >= (t.page_size ? 16 * kUnits : plan.target) || room <= plan.least) plan.target = 0;
@@ -1239,6 +1249,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     if (plan.rows == 16) launch_shape<TYPE, DP, 16, 1, 4>(p, plan, s);
+    else if (plan.rows == 32) launch_shape<TYPE, DP, 32, 1, 4>(p, plan, s);
     else if (plan.rows == 128) launch_shape<TYPE, DP, 32, 4, 1>(p, plan, s);
     else launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
 }

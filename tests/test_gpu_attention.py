@@ -290,6 +290,32 @@ def test_paged_shapes(qmv, hip, t, heads, kv_heads, dim, new, length):
         _check(o[a:a + n][rows], ref, bound, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim} sequence {s} ({n} of {length[s]})")
 
 
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("heads,kv_heads,dim,count,longest", [(28, 4, 128, 24, 700), (14, 2, 64, 60, 200), (6, 1, 40, 12, 5000)])
+def test_paged_few_tokens_each(qmv, hip, t, heads, kv_heads, dim, count, longest):
+    """Sequences of 17 to 32 rows on average, as when a few drafted tokens are
+    checked at once: some idle, some of one token, some of several row tiles,
+    one that stands partly before its first key, and a value that is not
+    finite, which only the rows that attend it may see."""
+    rng = np.random.default_rng(21)
+    new = [int(x) for x in rng.choice([4, 4, 4, 3, 5, 1, 0, 9], count)]
+    new[:4] = [5, 4, 9, 4]
+    length = [int(n + x) for n, x in zip(new, rng.integers(0, longest, count))]
+    length[0], length[1], length[2] = longest, 2, 9
+    assert 17 <= sum(new) * (heads // kv_heads) / count <= 32
+    b, q, keys, values, _ = _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, 16, seed=22)
+    odd = [x.copy() for x in values]
+    odd[3][length[3] - 2, 0, 5] = np.inf  # the third of four new tokens
+    o, ok = _paged(qmv, hip, b, q, A.Cache(qmv, hip, b, keys, odd, t), dim ** -0.5, 4, 8)
+    assert ok == 1
+    a, first = int(b.starts[3]), heads // kv_heads
+    assert not np.isfinite(o[a + 2:a + 4, :first, 5]).any()
+    ref, _ = A.attention64(q[a + 2:a + 4], keys[3], values[3], dim ** -0.5, b.positions(3)[2:])
+    o[a + 2:a + 4, :first, 5] = ref[:, :first, 5]
+    assert (o[int(b.starts[1]):int(b.starts[1]) + 2] == 0).all()
+    _check_paged(b, q, keys, values, o, dim ** -0.5, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim}")
+
+
 @pytest.mark.parametrize("count,longest", [(139, 200), (257, 40), (2500, 30)])
 def test_paged_many_sequences(qmv, hip, count, longest):
     """More sequences than a wave has lanes, or than workgroups look through
