@@ -1232,18 +1232,28 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     return plan;
 }
 
+template <int DP, int ROWS, int GROUPS> static void launch_join(const AttnParams &p, const AttnPlan &plan, float down, hipStream_t s)
+{
+    constexpr int EACH = 256 / (DP / 4 * GROUPS); /* rows of a workgroup */
+    /* workgroups of a tile for the rows that a sequence has on average */
+    const int64_t each = ((int64_t)p.t.tokens * (p.t.heads / p.t.kv_heads) + p.t.count - 1) / p.t.count;
+    const int slices = (int)(((each < ROWS ? each : ROWS) + EACH - 1) / EACH);
+    const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * slices);
+    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices, down);
+}
+
 template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
     if (plan.lists) attention_list_kernel<S::ROWS, S::KT * WK><<<1, 1024, 0, s>>>(p);
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
-    constexpr int ROWS = RW * WR, GROUPS = ROWS == 16 ? 8 : 1, EACH = 256 / (DP / 4 * GROUPS);
-    /* of a tile of 16, workgroups for the rows that a sequence has on average */
-    const int64_t each = ((int64_t)p.t.tokens * (p.t.heads / p.t.kv_heads) + p.t.count - 1) / p.t.count;
-    const int slices = (int)(((ROWS == 16 && each < ROWS ? each : ROWS) + EACH - 1) / EACH);
-    const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * slices);
-    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices, TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f);
+    const float down = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f;
+    /* Groups of threads where a tile has many pieces (the tiles counted here are an
+     * upper bound): 4 tokens over 32000 keys 31 us, 48 with one group; 64 sequences
+     * of 1000 keys 34 with groups, 32 with one. */
+    if (plan.target >= 8 * plan.tiles * p.t.kv_heads) launch_join<DP, S::ROWS, 8>(p, plan, down, s);
+    else launch_join<DP, S::ROWS, 1>(p, plan, down, s);
 }
 
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
