@@ -644,17 +644,21 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int JOIN = WK > 1 ? WK * (RW * DP * 4) : 0; /* the waves' O, where they meet */
     static constexpr int TILES = IMAGE ? 2 : WK;
     static constexpr int LDS = TILES * TILE > JOIN ? TILES * TILE : JOIN;
-    static constexpr int PARTIAL = ROWS * DP + 2 * ROWS;    /* floats of a piece's result */
 };
 
-/* From 32 rows on two waves a SIMD (except where two limbs of 128 elements and
- * their loads do not fit 256 registers beside 32 rows of a wave: 38 would spill;
- * with one, of f16 keys, 32 rows take 149 us for 4 tokens each over 64 sequences
- * of 4000, and 112 with two). At 16 and 32 rows the 4 waves have a tile each in
- * their own LDS and need no barrier. */
-template <int TYPE, int DP, int RW, int WR, int WK>
-__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (RW == 32 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
-void attention_kernel(AttnParams p)
+template <class S, int DP, int RW, int WK> struct AttnShared {
+    __attribute__((aligned(16))) unsigned char lds[S::LDS];
+    /* of the keys: factors; of the values: exponents; of an image: its whole head */
+    float scales[S::TILES][S::IMAGE ? kImageHead : 2 * S::NB];
+    int first_odd[DP]; /* the first key whose value is not finite there */
+    int any_odd;
+    float joined[WK > 1 ? WK : 1][2][RW];
+};
+
+/* One piece; LAYOUT: rows of a tile as its result's place in the workspace. */
+template <int TYPE, int DP, int RW, int WR, int WK, int LAYOUT>
+__device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem &it, int item, int kvh,
+                                             AttnShared<AttnShape<TYPE, DP, RW, WR, WK>, DP, RW, WK> &shared)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
     using P = Product<RW>;
@@ -663,23 +667,17 @@ void attention_kernel(AttnParams p)
     constexpr int KT = S::KT, NB = S::NB, UNITS = S::UNITS, SLOTS = S::SLOTS, MAT = S::MAT, NL = S::NL;
     constexpr int THREADS = 64 * WR * WK, WIDE = 512 / RW; /* of a product's contraction */
     constexpr int STEPS = DP / WIDE, DB = DP / RW, REGS = RW * RW / 64, SCORES = RW / 2;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[S::LDS];
-    /* of the keys: factors; of the values: exponents; of an image: its whole head */
-    __shared__ float scales[S::TILES][IMAGE ? kImageHead : 2 * NB];
-    __shared__ int first_odd[DP]; /* the first key whose value is not finite there */
-    __shared__ int any_odd;
-    __shared__ float joined[WK > 1 ? WK : 1][2][RW];
+    constexpr int PARTIAL = LAYOUT * DP + 2 * LAYOUT; /* floats of a piece's result */
+    auto &lds = shared.lds;
+    auto &scales = shared.scales;
+    auto &first_odd = shared.first_odd;
+    auto &any_odd = shared.any_odd;
+    auto &joined = shared.joined;
 
     const AttnTokens &a = p.t;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, part_of = lane / RW, col = lane % RW;
     const int group = a.heads / a.kv_heads, dim = a.dim;
-    const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-    AttnItem it;
-    int tiles_all;
-    const bool found = find_item<S::ROWS, KT * WK>(p, item, lane, &it, &tiles_all);
-    if (blockIdx.x == 0 && p.target && tid == 0) p.joins[0].n = tiles_all;
-    if (!found) return;
     for (int i = tid; i < DP; i += THREADS) first_odd[i] = INT32_MAX;
     if (tid == 0) any_odd = 0;
     lds_barrier();
@@ -993,7 +991,7 @@ void attention_kernel(AttnParams p)
     }
     l = sum_lanes<RW>(l);
     constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
-    float *const part = p.partials + (int64_t)blockIdx.x * S::PARTIAL;
+    float *const part = p.partials + (int64_t)blockIdx.x * PARTIAL;
 
     if (WK == 1) {
         /* register 4 j + i of o[db]: element RW db + 8 j + 4 part_of + i of this lane's row */
@@ -1020,7 +1018,7 @@ void attention_kernel(AttnParams p)
             }
         if (pieces > 1 && part_of == 0) {
             const f2_t v = {r, l};
-            *(f2_t *)(part + S::ROWS * DP + 2 * row_in_tile) = v;
+            *(f2_t *)(part + LAYOUT * DP + 2 * row_in_tile) = v;
         }
     } else {
         /* the waves' results meet in LDS */
@@ -1069,11 +1067,48 @@ void attention_kernel(AttnParams p)
                 *(f4_t *)(part + rr * DP + 4 * d4) = v;
                 if (d4 == 0) {
                     const f2_t st = {all, sum};
-                    *(f2_t *)(part + S::ROWS * DP + 2 * rr) = st;
+                    *(f2_t *)(part + LAYOUT * DP + 2 * rr) = st;
                 }
             }
         }
     }
+}
+
+/* From 32 rows on two waves a SIMD (except where two limbs of 128 elements and
+ * their loads do not fit 256 registers beside 32 rows of a wave: 38 would spill;
+ * with one, of f16 keys, 32 rows take 149 us for 4 tokens each over 64 sequences
+ * of 4000, and 112 with two). At 16 and 32 rows the 4 waves have a tile each in
+ * their own LDS and need no barrier. */
+template <int TYPE, int DP, int RW, int WR, int WK>
+__global__ __launch_bounds__(64 * WR * WK, WR == 8 || (RW == 32 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
+void attention_kernel(AttnParams p)
+{
+    using S = AttnShape<TYPE, DP, RW, WR, WK>;
+    using Few = AttnShape<TYPE, DP, 16, 1, 4>;
+    using Shared = AttnShared<S, DP, RW, WK>;
+    using FewShared = AttnShared<Few, DP, 16, 4>;
+    constexpr bool MIXED = S::ROWS == 128;
+    constexpr size_t BYTES = MIXED && sizeof(FewShared) > sizeof(Shared) ? sizeof(FewShared) : sizeof(Shared);
+    __shared__ __attribute__((aligned(16))) unsigned char memory[BYTES];
+
+    const AttnTokens &a = p.t;
+    const int kvh = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+    AttnItem it;
+    int tiles_all;
+    const bool found = find_item<S::ROWS, S::KT * WK>(p, item, threadIdx.x & 63, &it, &tiles_all);
+    if (blockIdx.x == 0 && p.target && threadIdx.x == 0) p.joins[0].n = tiles_all;
+    if (!found) return;
+    /* A decoding sequence among longer ones: its one tile as the 16-row kernel
+     * takes it (512 tokens and 15 decoding sequences of 8000 keys 106 us without, 71
+     * with; 28 and 4 heads of 128, f16). That has its place in LDS beside two
+     * workgroups a compute unit, and no more registers than 128 rows. */
+    if constexpr (MIXED) {
+        if (it.n * (a.heads / a.kv_heads) <= 16) {
+            attend_piece<TYPE, DP, 16, 1, 4, S::ROWS>(p, it, item, kvh, *(FewShared *)memory);
+            return;
+        }
+    }
+    attend_piece<TYPE, DP, RW, WR, WK, S::ROWS>(p, it, item, kvh, *(Shared *)memory);
 }
 
 /* Joins the pieces of rows whose keys were cut, in their order within each of

@@ -316,6 +316,24 @@ def test_paged_few_tokens_each(qmv, hip, t, heads, kv_heads, dim, count, longest
     _check_paged(b, q, keys, values, o, dim ** -0.5, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim}")
 
 
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(28, 4, 128), (14, 2, 64), (6, 1, 40)])
+def test_paged_decoding_beside_chunks(qmv, hip, t, heads, kv_heads, dim):
+    """A step of a server: chunks of prompts and decoding sequences in one call,
+    with a value that is not finite, which only the second of two tokens sees."""
+    new, length = [60, 1, 0, 2, 20, 1, 1, 4], [400, 4000, 5, 700, 40, 1, 1290, 31]
+    b, q, keys, values, _ = _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, 16, seed=23)
+    odd = [x.copy() for x in values]
+    odd[3][699, 0, 5] = np.nan
+    o, ok = _paged(qmv, hip, b, q, A.Cache(qmv, hip, b, keys, odd, t), dim ** -0.5, 4, 8)
+    assert ok == 1
+    a, group = int(b.starts[3]) + 1, heads // kv_heads
+    assert np.isnan(o[a, :group, 5]).all()
+    ref, _ = A.attention64(q[a:a + 1], keys[3], values[3], dim ** -0.5, [699])
+    o[a, :group, 5] = ref[0, :group, 5]
+    _check_paged(b, q, keys, values, o, dim ** -0.5, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim}")
+
+
 @pytest.mark.parametrize("count,longest", [(139, 200), (257, 40), (2500, 30)])
 def test_paged_many_sequences(qmv, hip, count, longest):
     """More sequences than a wave has lanes, or than workgroups look through
