@@ -364,8 +364,9 @@ __device__ __forceinline__ float work_of(const AttnTokens &a, const AttnSequence
 }
 
 /* Keys of a piece at most, from the sums over all sequences and the longest
- * that brings tokens; a whole wave asks. The sums are of floats, whose rounding
- * the one piece beyond plan_attention's count allows for.
+ * that brings tokens; `even`: their new tokens are alike. A whole wave asks. The
+ * sums are of floats, whose rounding the one piece beyond plan_attention's count
+ * allows for.
  *
  * Where the lengths are alike (and slots is set: up to 32 rows over f16 or bf16) each
  * lane takes a number of pieces per tile and says what it costs: rounds of the
@@ -374,12 +375,13 @@ __device__ __forceinline__ float work_of(const AttnTokens &a, const AttnSequence
  * streams up to 1 / 0.58 times as fast as two. 28 and 4 heads of 128, f16, with
  * and without (us): 64 sequences of 1000 keys 33 / 42, of 4000 108 / 121, 16 of
  * 4000 33 / 41. */
-template <int STEP> __device__ __forceinline__ int chunk_of(const AttnParams &p, float work, float tiles, int longest)
+template <int STEP> __device__ __forceinline__ int chunk_of(const AttnParams &p, float work, float tiles, int longest, bool even)
 {
     const int whole = INT32_MAX / STEP * STEP;
     if (p.target == 0) return whole;
-    const int pieces = p.target / p.t.kv_heads;
-    if (p.slots && tiles * (float)longest <= 1.1f * work && tiles * 64.f >= (float)pieces) {
+    const bool alike = even && tiles * (float)longest <= 1.1f * work;
+    const int pieces = (alike ? p.alike : p.target) / p.t.kv_heads;
+    if (p.slots && alike && tiles * 64.f >= (float)pieces) {
         const int lane = threadIdx.x & 63, n = lane + 1;
         const int keys = max((longest / n + STEP) / STEP * STEP, STEP); /* n of them reach `longest` */
         const float items = tiles * (float)n, load = items * (float)p.t.kv_heads / (float)p.slots;
@@ -440,11 +442,13 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
         return true;
     }
     AttnSequence q;
-    float work = 0.f, rows = 0.f, tiles = 0.f;
-    int longest = 0;
+    float work = 0.f, rows = 0.f, tiles = 0.f, busy = 0.f;
+    int longest = 0, most = 0;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
         q = sequence_at<BM>(a, s0 + lane);
         longest = max(longest, q.n > 0 ? q.len : 0);
+        most = max(most, q.n);
+        busy += q.n > 0 ? 1.f : 0.f;
         work += work_of(a, q);
         rows += (float)q.n;
         tiles += (float)q.tiles;
@@ -454,7 +458,9 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
     tiles = lane_of(scan_lanes(tiles), 63);
     *tiles_all = 0;
     if (rows > (float)a.tokens) return false;
-    const int chunk = chunk_of<STEP>(p, work, tiles, (int)wave_max((uint32_t)longest));
+    bool even = true;
+    if (p.alike != p.target) even = (float)wave_max((uint32_t)most) * lane_of(scan_lanes(busy), 63) <= 1.1f * rows;
+    const int chunk = chunk_of<STEP>(p, work, tiles, (int)wave_max((uint32_t)longest), even);
     int before = 0, tiles_before = 0;
     bool found = false;
     for (int s0 = 0; s0 < a.count; s0 += 64) {
@@ -485,15 +491,17 @@ __device__ __forceinline__ bool find_item(const AttnParams &p, int item, int lan
  * 28 and 4 heads: 9.7 ms without.) */
 template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_list_kernel(AttnParams p)
 {
-    __shared__ float sums[3][16];
-    __shared__ int longests[16], ends[1024], tile_ends[16], item_ends[16];
+    __shared__ float sums[4][16];
+    __shared__ int longests[16], mosts[16], ends[1024], tile_ends[16], item_ends[16];
     const AttnTokens &a = p.t;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float work = 0.f, rows = 0.f, tiles = 0.f;
-    int longest = 0;
+    float work = 0.f, rows = 0.f, tiles = 0.f, busy = 0.f;
+    int longest = 0, most = 0;
     for (int s = tid; s < a.count; s += 1024) {
         const AttnSequence q = sequence_at<BM>(a, s);
         longest = max(longest, q.n > 0 ? q.len : 0);
+        most = max(most, q.n);
+        busy += q.n > 0 ? 1.f : 0.f;
         work += work_of(a, q);
         rows += (float)q.n;
         tiles += (float)q.tiles;
@@ -501,22 +509,28 @@ template <int BM, int STEP> __global__ __launch_bounds__(1024) void attention_li
     work = scan_lanes(work);
     rows = scan_lanes(rows);
     tiles = scan_lanes(tiles);
+    busy = scan_lanes(busy);
     longest = (int)wave_max((uint32_t)longest);
+    most = (int)wave_max((uint32_t)most);
     if (lane == 63) {
         longests[wave] = longest;
+        mosts[wave] = most;
+        sums[3][wave] = busy;
         sums[0][wave] = work;
         sums[1][wave] = rows;
         sums[2][wave] = tiles;
     }
     __syncthreads();
-    work = rows = tiles = 0.f;
+    work = rows = tiles = busy = 0.f;
     for (int i = 0; i < 16; ++i) {
         work += sums[0][i];
         rows += sums[1][i];
         tiles += sums[2][i];
+        busy += sums[3][i];
         longest = max(longest, longests[i]);
+        most = max(most, mosts[i]);
     }
-    const int chunk = chunk_of<STEP>(p, work, tiles, longest);
+    const int chunk = chunk_of<STEP>(p, work, tiles, longest, (float)most * busy <= 1.1f * rows || p.alike == p.target);
     const bool valid = rows <= (float)a.tokens;
     int items_before = 0, tiles_before = 0;
     for (int s0 = 0; valid && s0 < a.count; s0 += 1024) {
@@ -1217,7 +1231,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
  * 32 and 128 rows and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152 with
  * 512); of 16 rows twice that, because sequences that decode differ in length
  * most (64 of 1 to 8191 keys: 110 with 1024, 123 with 512), except over fp32,
- * whose tiles leave room for one workgroup.
+ * whose tiles leave room for one workgroup. Also twice over a cache where tiles
+ * of 128 alone are more than half of them, unless lengths and new tokens are alike
+ * (which the device sees): 512 tokens and 63 decoding sequences of 4000 keys 170 and 223, 6
+ * tokens each over 10 to 6310 keys in 64 sequences 150 and 206, but 64 tokens each
+ * over 1000 in 16 sequences 75 and 64.
  * Images: 5 us for their kernel, against splitting a key once per row tile: 1024
  * tokens per prompt are 28 tiles (7B), where both take the same time. */
 AttnPlan plan_attention(const AttnTokens &t, int type)
@@ -1236,6 +1254,8 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     plan.tiles = (int)tiles;
 
     plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows != 16 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
+    plan.alike = plan.target;
+    if (plan.rows == 128 && t.page_size && 2 * tiles * heads > plan.target) plan.target *= 2;
     plan.slots = plan.rows <= 32 && t.page_size && type != QMV_KV_F32 ? (int)(2 * kUnits) : 0;
     plan.least = plan.rows <= 32 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
     /* None where the tiles are enough (a cache's sequences may still differ in

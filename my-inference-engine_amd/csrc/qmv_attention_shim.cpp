@@ -234,6 +234,7 @@ try {
     if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + joins + plan.lists)) return 0;
     unsigned char *at = ws.data;
     p.target = plan.target;
+    p.alike = plan.alike;
     p.least = plan.least;
     p.slots = plan.slots;
     p.image = at;

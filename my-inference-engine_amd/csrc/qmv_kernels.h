@@ -174,6 +174,7 @@ struct AttnParams {
     /* Work of few rows is cut along the keys into about `target` pieces (0:
      * not), whose partial results meet in the workspace. */
     int target;
+    int alike; /* the same of sequences whose lengths and new tokens are alike */
     int least; /* keys of a piece at least, whole steps of the kernel */
     int slots; /* workgroups that run at once, 0: the pieces are not fitted to them */
     float *partials;
@@ -191,7 +192,7 @@ struct AttnParams {
  * workgroups and the workspace. */
 struct AttnPlan {
     int rows;
-    int target, least, slots;
+    int target, alike, least, slots;
     int tiles; /* row tiles at most, of one key head */
     int64_t grid;
     int items;              /* pieces at most, of one key head */

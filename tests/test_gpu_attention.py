@@ -334,6 +334,26 @@ def test_paged_decoding_beside_chunks(qmv, hip, t, heads, kv_heads, dim):
     _check_paged(b, q, keys, values, o, dim ** -0.5, f"{A.NAMES[t]} {heads}/{kv_heads}/{dim}")
 
 
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("heads,kv_heads,new,length", [
+    (28, 4, [240] + [1] * 60, [240] + [(37 * i) % 700 + 1 for i in range(60)]),  # decoding beside a prompt
+    (28, 4, [6] * 60, [500 + i % 9 for i in range(60)]),                         # all alike
+    (7, 1, [5] * 300, [5 + 7 * i % 90 for i in range(300)]),                     # more than workgroups look through themselves
+])
+def test_paged_many_tiles(qmv, hip, t, heads, kv_heads, new, length):
+    """Tiles of 128 rows that are nearly as many as the workgroups at once."""
+    b, q, keys, values, cache = _paged_case(qmv, hip, new, length, heads, kv_heads, 128, t, 16, seed=24)
+    o, ok = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
+    assert ok == 1
+    for s, n in enumerate(new):
+        a, rows = int(b.starts[s]), sorted({0, 17, 18, 36, n // 2, n - 1} & set(range(n)))
+        pos = b.positions(s)
+        ref, bound = A.attention64(q[a:a + n][rows], keys[s], values[s], 128 ** -0.5, [pos[i] for i in rows])
+        assert (np.abs(o[a:a + n][rows] - ref) <= bound).all(), (s, n, length[s])
+    again, _ = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
+    assert np.array_equal(o.view(np.uint32), again.view(np.uint32))
+
+
 @pytest.mark.parametrize("count,longest", [(139, 200), (257, 40), (2500, 30)])
 def test_paged_many_sequences(qmv, hip, count, longest):
     """More sequences than a wave has lanes, or than workgroups look through
