@@ -8,12 +8,12 @@
  * What bounds attention (28 query and 4 key heads of 128 unless said; a copy
  * reaches 4.6 TB/s here and an 8192^3 f16 product 1.1 PFLOP/s):
  *   one token each of 64 sequences of 1 to 8191 keys, f16 cache: the stream of
- *   keys and values, 494 MB in 110 us with the join, 4.5 TB/s;
+ *   keys and values, 494 MB in 98 us with the join, 5.0 TB/s;
  *   a prompt of 8192: the matrix cores, 1.44 T operations (three products of
- *   limbs each) in 1.29 ms, 1.12 PFLOP/s at 2.0 GHz, where the power limit holds
+ *   limbs each) in 1.24 to 1.29 ms, 1.12 PFLOP/s at 2.0 GHz, where the power limit holds
  *   the clock;
  *   512 tokens over 16100, f16 cache: the matrix cores, 0.23 T (two products) in
- *   251 us, 0.93 PFLOP/s with the pieces' results and their join;
+ *   247 us, 0.94 PFLOP/s with the pieces' results and their join;
  *   small calls: their chain of memory round trips (lengths, page table, keys)
  *   and a second launch for the join: one token over 777 keys, 14 and 2 heads of
  *   64, 9 + 3 us.
