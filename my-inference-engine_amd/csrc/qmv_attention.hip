@@ -1101,7 +1101,7 @@ void attention_kernel(AttnParams p)
     using Few = AttnShape<TYPE, DP, 16, 1, 4>;
     using Shared = AttnShared<S, DP, RW, WK>;
     using FewShared = AttnShared<Few, DP, 16, 4>;
-    constexpr bool MIXED = S::ROWS == 128;
+    constexpr bool MIXED = S::ROWS >= 128 && !S::IMAGE;
     constexpr size_t BYTES = MIXED && sizeof(FewShared) > sizeof(Shared) ? sizeof(FewShared) : sizeof(Shared);
     __shared__ __attribute__((aligned(16))) unsigned char memory[BYTES];
 
@@ -1114,10 +1114,12 @@ void attention_kernel(AttnParams p)
     if (!found) return;
     /* A decoding sequence among longer ones: its one tile as the 16-row kernel
      * takes it (512 tokens and 15 decoding sequences of 8000 keys 106 us without, 71
-     * with; 28 and 4 heads of 128, f16). That has its place in LDS beside two
-     * workgroups a compute unit, and no more registers than 128 rows. */
+     * with, 2048 and 8 of 6000 182 and 133; 28 and 4 heads of 128, f16). That has its
+     * place in LDS beside the workgroups that run at once, and needs no more
+     * registers (of fp32 under 256 rows 16 spill). */
     if constexpr (MIXED) {
         if (it.n * (a.heads / a.kv_heads) <= 16) {
+            if (threadIdx.x >= 256) return; /* a barrier waits for the waves that are left */
             attend_piece<TYPE, DP, 16, 1, 4, S::ROWS>(p, it, item, kvh, *(FewShared *)memory);
             return;
         }
@@ -1232,10 +1234,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
  * 512); of 16 rows twice that, because sequences that decode differ in length
  * most (64 of 1 to 8191 keys: 110 with 1024, 123 with 512), except over fp32,
  * whose tiles leave room for one workgroup. Also twice over a cache where tiles
- * of 128 alone are more than half of them, unless lengths and new tokens are alike
+ * of 128 or 256 alone are more than half of them, unless lengths and new tokens are alike
  * (which the device sees): 512 tokens and 63 decoding sequences of 4000 keys 170 and 223, 6
- * tokens each over 10 to 6310 keys in 64 sequences 150 and 206, but 64 tokens each
- * over 1000 in 16 sequences 75 and 64.
+ * tokens each over 10 to 6310 keys in 64 sequences 150 and 206, 1024 tokens
+ * and 40 of 1 to 7801 keys of fp32 299 and 380, but 64 tokens each over 1000 in 16
+ * sequences 75 and 64.
  * Images: 5 us for their kernel, against splitting a key once per row tile: 1024
  * tokens per prompt are 28 tiles (7B), where both take the same time. */
 AttnPlan plan_attention(const AttnTokens &t, int type)
@@ -1255,7 +1258,7 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
 
     plan.target = (int)(plan.rows == 256 ? kUnits : plan.rows != 16 || type == QMV_KV_F32 ? 2 * kUnits : 4 * kUnits);
     plan.alike = plan.target;
-    if (plan.rows == 128 && t.page_size && 2 * tiles * heads > plan.target) plan.target *= 2;
+    if (plan.rows >= 128 && t.page_size && 2 * tiles * heads > plan.target) plan.target *= 2;
     plan.slots = plan.rows <= 32 && t.page_size && type != QMV_KV_F32 ? (int)(2 * kUnits) : 0;
     plan.least = plan.rows <= 32 && type != QMV_KV_F32 ? 256 : 128; /* keys, 64 KB of 128 elements */
     /* None where the tiles are enough (a cache's sequences may still differ in

@@ -338,10 +338,13 @@ def test_paged_decoding_beside_chunks(qmv, hip, t, heads, kv_heads, dim):
 @pytest.mark.parametrize("heads,kv_heads,new,length", [
     (28, 4, [240] + [1] * 60, [240] + [(37 * i) % 700 + 1 for i in range(60)]),  # decoding beside a prompt
     (28, 4, [6] * 60, [500 + i % 9 for i in range(60)]),                         # all alike
+    (28, 4, [600, 1, 2], [700, 2500, 1200]),                                     # tiles of 256 rows
+    (28, 4, [900] + [1] * 20, [900] + [90 * i + 1 for i in range(20)]),          # of fp32 alone
     (7, 1, [5] * 300, [5 + 7 * i % 90 for i in range(300)]),                     # more than workgroups look through themselves
 ])
 def test_paged_many_tiles(qmv, hip, t, heads, kv_heads, new, length):
-    """Tiles of 128 rows that are nearly as many as the workgroups at once."""
+    """Tiles of 128 or 256 rows that are nearly as many as the workgroups at once,
+    decoding sequences among them."""
     b, q, keys, values, cache = _paged_case(qmv, hip, new, length, heads, kv_heads, 128, t, 16, seed=24)
     o, ok = _paged(qmv, hip, b, q, cache, 128 ** -0.5)
     assert ok == 1
