@@ -12,7 +12,6 @@ Activations are fp32, as the projections leave them; a cache holds f32, f16 or
 bf16. `heads` and `kv_heads` are those of queries and of keys; `new` lists how
 many tokens each sequence brings, `length` how many it then has.
 """
-import functools
 import importlib
 import math
 
@@ -163,14 +162,8 @@ def prepare(case, seed):
 # ---- one pass ------------------------------------------------------------------------
 
 
-@functools.cache
-def _package():
-    """The library, imported once as a program does"""
-    return importlib.import_module("my-inference-engine_amd")
-
-
 def _own(state):
-    qmv = _package()
+    qmv = importlib.import_module("my-inference-engine_amd")
     case, stream = state["case"], torch.cuda.current_stream().cuda_stream
     heads, kv_heads, dim, tokens = case["heads"], case["kv_heads"], case["dim"], state["tokens"]
     if case["kind"] == "prompt":
