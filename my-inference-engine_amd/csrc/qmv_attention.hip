@@ -1360,7 +1360,7 @@ template <int TYPE> __global__ __launch_bounds__(256) void rope_kernel(RopeParam
     const int t = blockIdx.x, half = p.rotary / 2, dim = a.dim;
     const int s = sequence_of(a, t);
     if (s < 0) return;
-    const int start = a.starts[s], n = min(a.starts[s + 1], a.tokens) - start;
+    const int start = max(a.starts[s], 0), n = min(a.starts[s + 1], a.tokens) - start; /* start <= t < tokens */
     const int pos = (a.lengths ? a.lengths[s] - n : 0) + t - start;
     for (int i = threadIdx.x; i < half; i += 256) {
         const double angle = (double)pos * p.freq[i];
