@@ -195,7 +195,7 @@ template <typename T> __device__ __forceinline__ T lane_of(T v, int lane)
  * than 2^4 over it, so that most tiles leave O as it is. */
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNothing = -3.0e38f; /* r before any key */
+constexpr float kNothing = -3.40282347e38f; /* r before any key: no finite score is below it */
 constexpr float kShift = 11.f;       /* weights are at most 2^(kShift + kSlack) */
 constexpr float kSlack = 4.f;
 

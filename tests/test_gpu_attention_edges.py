@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import _attention as A
-from test_gpu_attention import _rand, _rope_bound, hip  # noqa: F401
+from test_gpu_attention import _prompt, _rand, _rope_bound, hip  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +31,23 @@ def test_rope_cuts_starts_to_the_tokens(qmv, hip, with_lengths):  # noqa: F811
     for got, x in ((qo.to_array(np.float32, q.shape), q), (ko.to_array(np.float32, k.shape), k)):
         for t, p in enumerate(positions):
             assert np.max(np.abs(got[t] - A.rope64(x[t], p, f, False))) <= _rope_bound(x[t]), (t, p)
+
+
+# ---- scores at the ends of the range -----------------------------------------------------
+
+
+def test_scores_far_below_zero(qmv, hip):  # noqa: F811
+    """Rows whose scores all lie near the lowest fp32 number (here -2.3e38, in
+    powers of two -3.3e38) are averages like any others. Keys alike, so that the
+    weights are: the result is the mean of the values, each held to 2^-22 of
+    itself (their sizes are alike), the weights too, and the sums of n terms
+    rounded by at most n 2^-23 of them."""
+    rng = np.random.default_rng(41)
+    for n, dim in ((1, 64), (70, 64), (70, 128)):
+        q, k = np.zeros((n, 2, dim), np.float32), np.zeros((n, 1, dim), np.float32)
+        q[..., 3], k[..., 3] = 1.5e19, -1.533e19
+        v = _rand(rng, n, 1, dim)
+        o = _prompt(qmv, hip, [n], 2, 1, dim, q, k, v, 1.0)
+        for i in range(n):
+            ref, size = v[:i + 1, 0].astype(np.float64).mean(0), np.abs(v[:i + 1, 0]).astype(np.float64).mean(0)
+            assert (np.abs(o[i] - ref) <= (2 * 2.0 ** -22 + 2 * (i + 1) * 2.0 ** -23 + 2.0 ** -22) * size).all(), (n, dim, i)
