@@ -450,10 +450,17 @@ int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride,
  * length is never used.
  *
  * Both forms multiply on the matrix cores with fp32 sums. q, the weights, and
- * keys and values of fp32 are two f16 limbs, held to 2^-22 of themselves, or to
- * 2^-39 of the largest of a row of q or of 16 consecutive tokens of a head,
- * where that is more; keys and values of bf16 exactly or to that 2^-39; those
- * of f16 exactly. Magnitudes below 2^-110 lose places. A key that is not finite
+ * keys and values of fp32 are two f16 limbs, each held to 2^-22 of itself or,
+ * where that is more, to
+ *   q: 2^-39 of the largest of its row;
+ *   weights: 2^-25 of the row's largest;
+ *   keys and values of fp32 and bf16: 2^-39 of the largest of 16 consecutive
+ *   tokens of a head (bf16 is exact but for that; f16 is exact).
+ * Magnitudes below 2^-110 lose places, and so do products of a weight and a
+ * value below 2^-60 of a row's largest. The weights' sum is of fp32. Where the
+ * values of a row's blocks of 16 tokens differ by more than 2^10 in size, the
+ * products take about twice the time.
+ * A key that is not finite
  * makes the rows that attend it NaN, a value the elements that sum it not
  * finite; neither reaches other rows.
  * The work of few rows is cut along the length and joined in a fixed order: the

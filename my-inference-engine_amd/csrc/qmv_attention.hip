@@ -191,12 +191,30 @@ template <typename T> __device__ __forceinline__ T lane_of(T v, int lane)
  * scores; that of the values is added to the exponents of its weights, and
  * taken out again where the weights are summed.
  *
- * The weights' reference r follows the running maximum only when that is more
- * than 2^4 over it, so that most tiles leave O as it is. */
+ * Two references, both whole numbers, so that moving them rounds nothing: the
+ * weights' sum l is of 2^(score - m - 9), m following the running maximum of
+ * the scores; O is relative to 2^(m + rm), which follows that of score plus the
+ * exponent of a block's values. (Of f16 values, which have no exponents, one
+ * reference r is both.) They move only when the maximum is more than 2^4 over
+ * them, so that most tiles leave O as it is.
+ *
+ * Where the values of a row's blocks differ much in size (by more than 2^kApart
+ * between their largest), the smaller ones' weights would lose places in limbs
+ * beside the larger's reference. From there on a wave takes the blocks one after
+ * the other, each relative to its own largest: O is brought down to that
+ * reference and the next block's raises it again, exactly, down to 2^-kReach of
+ * the row's largest product of weight and value so far; products below that are
+ * left out of O, their weights still summed in l. The same where scores are so
+ * large (2^22) that an exponent added to them would be rounded away. Against one
+ * reference for both, which left l to the weights of the largest values (values
+ * of 1e30 beside zeros: off by any factor; one channel of 2^30 in 16 tokens: the
+ * others off by 1e-2): 1.3 to 1.7% of a long prompt, 3% of the 0.5B prompts. */
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNothing = -3.40282347e38f; /* r before any key: no finite score is below it */
-constexpr float kShift = 11.f;       /* weights are at most 2^(kShift + kSlack) */
+constexpr float kNothing = -3.40282347e38f; /* r, m before any key: no finite score is below it */
+constexpr float kNoScale = -1000.f;         /* rm before any key */
+constexpr float kApart = 10.f, kReach = 60.f;
+constexpr float kShift = 11.f; /* weights are at most 2^(kShift + kSlack) */
 constexpr float kSlack = 4.f;
 
 /* 2^n as a float, -126 <= n <= 127. */
@@ -317,6 +335,7 @@ template <int DP> __device__ __forceinline__ int turn_of(int key)
     return DP == 128 ? (key & 3) << 2 | (key >> 2 & 3) : (key >> 1 & 1) << 2 | (key >> 2 & 3);
 }
 constexpr int kMostKeys = 126, kMostValues = 100; /* most factors of scale_of */
+constexpr int kZeroValues = 12; /* the factor of a block of zeros: what values near one have, so that they are not apart */
 
 struct AttnItem {
     int s, start, n, len; /* the sequence, its first token, new tokens and length (cut to its pages) */
@@ -629,7 +648,7 @@ template <int DP> __global__ __launch_bounds__(256) void attention_image_kernel(
             for (int i = 0; i < SLOTS; ++i) top = max(top, raw[values][i].top_finite());
             top = wave_max(top);
         }
-        const int n2 = scale_of(top, values ? kMostValues : kMostKeys);
+        const int n2 = values && top == 0 ? kZeroValues : scale_of(top, values ? kMostValues : kMostKeys);
         if (lane == 0) head[4 * values + b] = values ? (float)-n2 : power_of_two(-n2);
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
@@ -658,6 +677,7 @@ template <int TYPE, int DP, int RW, int WR, int WK> struct AttnShape {
     static constexpr int JOIN = WK > 1 ? WK * (RW * DP * 4) : 0; /* the waves' O, where they meet */
     static constexpr int TILES = IMAGE ? 2 : WK;
     static constexpr int LDS = TILES * TILE > JOIN ? TILES * TILE : JOIN;
+    static constexpr int PEAKS = TYPE == QMV_KV_F16 ? 1 : WR * WK * RW;
 };
 
 template <class S, int DP, int RW, int WK> struct AttnShared {
@@ -667,6 +687,9 @@ template <class S, int DP, int RW, int WK> struct AttnShared {
     int first_odd[DP]; /* the first key whose value is not finite there */
     int any_odd;
     float joined[WK > 1 ? WK : 1][2][RW];
+    /* Each row's highest rm so far, where blocks are taken one after the other;
+     * a row's lanes write the same. */
+    float peaks[S::PEAKS];
 };
 
 /* One piece; LAYOUT: rows of a tile as its result's place in the workspace. */
@@ -687,6 +710,8 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
     auto &first_odd = shared.first_odd;
     auto &any_odd = shared.any_odd;
     auto &joined = shared.joined;
+    constexpr bool SCALED = TYPE != QMV_KV_F16;
+    float *const peak = shared.peaks + (SCALED ? (threadIdx.x >> 6) * RW + threadIdx.x % RW : 0);
 
     const AttnTokens &a = p.t;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -694,6 +719,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
     const int group = a.heads / a.kv_heads, dim = a.dim;
     for (int i = tid; i < DP; i += THREADS) first_odd[i] = INT32_MAX;
     if (tid == 0) any_odd = 0;
+    if (SCALED) *peak = kNoScale;
     lds_barrier();
 
     /* the keys of this piece */
@@ -788,7 +814,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
                     top = wave_max(top);
                 }
                 if (TYPE != QMV_KV_F16) {
-                    n = scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? kMostValues : kMostKeys);
+                    n = values && top == 0 ? kZeroValues : scale_of(TYPE == QMV_KV_BF16 ? top << 16 : top, values ? kMostValues : kMostKeys);
                     if (lane == 0) scales[wk][values ? NB + b : b] = values ? (float)-n : power_of_two(-n);
                 }
             }
@@ -863,7 +889,8 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
     acc_t o[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = acc_t{0};
-    float r = kNothing, l = 0.f;
+    float m = kNothing, rm = SCALED ? kNoScale : 0.f, l = 0.f; /* of f16 values m is r */
+    float limit = kNothing;                                    /* m + rm + kSlack */
     /* Key 32 sb + score_key(i) of a tile is the one of score register i. */
     auto score_key = [&](int i) { return (256 / RW) * (i >> 2) + 4 * part_of + (i & 3); };
     const int k_at = col * DP * 2 + ((part_of ^ turn_of<DP>(col)) << 4);
@@ -889,85 +916,134 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         const h4_t hx = __builtin_bit_cast(h4_t, x), hy = __builtin_bit_cast(h4_t, y);
         return h8_t{hx[0], hx[1], hx[2], hx[3], hy[0], hy[1], hy[2], hy[3]};
     };
+    constexpr int EACH = SCORES / 2; /* scores of a block of 16 keys */
+    constexpr int VS = 32 / WIDE;    /* steps of 8 scores a lane */
+    bool apart = false;
+    /* 32 keys; of blocks taken one after the other (apart) the first or the
+     * second. */
+    auto pass = [&](int k0, int sb, int only) {
+        /* Unknown to the compiler, so that it does not keep the masks of all
+         * scores between the two (93 spilled scalar registers at 128 rows). */
+        if (SCALED) asm volatile("" : "+s"(k0));
+        float c[SCORES];
+        __builtin_amdgcn_s_setprio(1); /* these products before the other waves' softmax: 1% of a long prompt */
+#pragma unroll
+        for (int kb = 0; kb < 32 / RW; ++kb) {
+            acc_t x = {0};
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st) {
+                const h8_t hi = k_frag(0, 32 / RW * sb + kb, st);
+                x = P::run(hi, qhi[st], x);
+                x = P::run(hi, qlo[st], x);
+                if (NL == 2) x = P::run(k_frag(1, 32 / RW * sb + kb, st), qhi[st], x);
+            }
+#pragma unroll
+            for (int i = 0; i < REGS; ++i) c[REGS * kb + i] = x[i];
+        }
+        __builtin_amdgcn_s_setprio(0);
+        const int first = k0 + 32 * sb;
+        const bool masked = first + 31 > unmasked;
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < SCORES; ++i)
+                if (first + score_key(i) > pos) c[i] = -INFINITY;
+        }
+        float by[2], add[2], most[2];
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            if (SCALED) {
+                /* within the finite positive floats, so that a masked score stays -inf */
+                by[g] = fminf(fmaxf(q_back * scales[buf][2 * sb + g], 1.1754944e-38f), 1.7014118e38f);
+                add[g] = scales[buf][NB + 2 * sb + g];
+            } else {
+                by[g] = q_back;
+                add[g] = 0.f;
+            }
+            most[g] = c[EACH * g];
+#pragma unroll
+            for (int i = 1; i < EACH; ++i) most[g] = fmaxf(most[g], c[EACH * g + i]);
+            top = fmaxf(top, fmaf(most[g], by[g], add[g]));
+        }
+        top = max_lanes<RW>(top);
+        const float low = fminf(add[0], add[1]);
+        float less = m; /* what the scores are taken relative to below */
+        if (apart || __any(top > limit || (SCALED && rm - low > kApart))) {
+            float to, fade;
+            if (SCALED) {
+                to = fmaxf(m, ceilf(max_lanes<RW>(fmaxf(most[0] * by[0], most[1] * by[1]))));
+                const float now = rm + (m - to);
+                float next = top > limit ? ceilf(top) - to : now;
+                apart = apart || __any(next - low > kApart || (fabsf(to) > 4194304.f && to > kNothing));
+                if (apart) {
+                    const float best = max_lanes<RW>(only ? most[1] * by[1] : most[0] * by[0]);
+                    const float own = ceilf(best) - to + (only ? add[1] : add[0]);
+                    const float high = fmaxf(fmaxf(*peak + (m - to), now), own);
+                    *peak = high;
+                    /* now: the row attends no key of the block */
+                    next = best == -INFINITY ? now : fmaxf(own, high - kReach);
+                    /* A block below the reach: its weights are kept large enough
+                     * for the sum, and are zero as f16. */
+                    const float lift = fminf(fmaxf(next - kReach - own, 0.f), 400.f);
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+                        for (int i = EACH * g; i < EACH * (g + 1); ++i) c[i] = g == only ? fmaf(c[i], by[g], -to) : -INFINITY;
+                        by[g] = 1.f;
+                        add[g] += lift;
+                    }
+                    less = 0.f;
+                } else {
+                    less = to;
+                }
+                fade = __builtin_amdgcn_exp2f(now - next); /* at most 2^kReach */
+                rm = next;
+            } else {
+                to = top > limit ? top : m;
+                fade = __builtin_amdgcn_exp2f(m - to);
+                less = to;
+            }
+            l *= __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            limit = m + rm + kSlack;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) o[i] *= fade;
+        }
+        h8_t phi[VS], plo[VS];
+        float w[SCORES];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const float over = add[g] - rm, shift = (over + kShift) - less;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = EACH * g; i < EACH * (g + 1); ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(c[i], by[g], shift));
+                sum += w[i];
+            }
+            l += SCALED ? __builtin_ldexpf(sum, -20 - (int)over) : sum; /* of zero weights zero */
+        }
+#pragma unroll
+        for (int g = 0; g < VS; ++g) {
+            limbs_of(w + 8 * g, &phi[g], &plo[g]);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const h8_t v = v_frag(0, VS * sb + g, db);
+                o[db] = P::run(v, phi[g], o[db]);
+                o[db] = P::run(v, plo[g], o[db]);
+                if (NL == 2) o[db] = P::run(v_frag(1, VS * sb + g, db), phi[g], o[db]);
+            }
+        }
+    };
     auto compute = [&](int k0) {
 #pragma unroll
         for (int sb = 0; sb < KT / 32; ++sb) {
             __builtin_amdgcn_sched_barrier(0);
-            float c[SCORES];
-            __builtin_amdgcn_s_setprio(1); /* these products before the other waves' softmax: 1% of a long prompt */
-#pragma unroll
-            for (int kb = 0; kb < 32 / RW; ++kb) {
-                acc_t x = {0};
-#pragma unroll
-                for (int st = 0; st < STEPS; ++st) {
-                    const h8_t hi = k_frag(0, 32 / RW * sb + kb, st);
-                    x = P::run(hi, qhi[st], x);
-                    x = P::run(hi, qlo[st], x);
-                    if (NL == 2) x = P::run(k_frag(1, 32 / RW * sb + kb, st), qhi[st], x);
-                }
-#pragma unroll
-                for (int i = 0; i < REGS; ++i) c[REGS * kb + i] = x[i];
-            }
-            __builtin_amdgcn_s_setprio(0);
-            const int first = k0 + 32 * sb;
-            const bool masked = first + 31 > unmasked;
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < SCORES; ++i)
-                    if (first + score_key(i) > pos) c[i] = -INFINITY;
-            }
-            float by[2], add[2], back[2];
-            float top = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                if (TYPE == QMV_KV_F16) {
-                    by[g] = q_back;
-                    add[g] = 0.f;
-                } else {
-                    /* within the finite positive floats, so that a masked score stays -inf */
-                    by[g] = fminf(fmaxf(q_back * scales[buf][2 * sb + g], 1.1754944e-38f), 1.7014118e38f);
-                    add[g] = scales[buf][NB + 2 * sb + g];
-                    back[g] = __builtin_ldexpf(1.f, -20 - (int)add[g]); /* may be a denormal */
-                }
-                constexpr int EACH = SCORES / 2; /* scores of a block of 16 keys */
-                float m = c[EACH * g];
-#pragma unroll
-                for (int i = 1; i < EACH; ++i) m = fmaxf(m, c[EACH * g + i]);
-                top = fmaxf(top, fmaf(m, by[g], add[g]));
-            }
-            top = max_lanes<RW>(top);
-            if (__any(top > r + kSlack)) {
-                const float to = top > r + kSlack ? top : r;
-                const float fade = __builtin_amdgcn_exp2f(r - to);
-                r = to;
-                l *= fade;
-#pragma unroll
-                for (int i = 0; i < DB; ++i) o[i] *= fade;
-            }
-            constexpr int VS = 32 / WIDE; /* steps of 8 scores a lane */
-            h8_t phi[VS], plo[VS];
-            float w[SCORES];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const float shift = add[g] - r + kShift;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = SCORES / 2 * g; i < SCORES / 2 * (g + 1); ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(fmaf(c[i], by[g], shift));
-                    sum += w[i];
-                }
-                l = TYPE == QMV_KV_F16 ? l + sum : fmaf(sum, back[g], l);
-            }
-#pragma unroll
-            for (int g = 0; g < VS; ++g) {
-                limbs_of(w + 8 * g, &phi[g], &plo[g]);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    const h8_t v = v_frag(0, VS * sb + g, db);
-                    o[db] = P::run(v, phi[g], o[db]);
-                    o[db] = P::run(v, plo[g], o[db]);
-                    if (NL == 2) o[db] = P::run(v_frag(1, VS * sb + g, db), phi[g], o[db]);
-                }
+            if constexpr (SCALED) {
+                int only = 0;
+                do pass(k0, sb, only);
+                while (apart && ++only < 2);
+            } else {
+                pass(k0, sb, 0);
             }
         }
     };
@@ -1004,7 +1080,15 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         }
     }
     l = sum_lanes<RW>(l);
-    constexpr float kDown = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f; /* 2^-20, as in l */
+    /* O to the sums themselves, together with the factor 1 / l */
+    const int back = SCALED ? (int)fminf(fmaxf(rm, -1000.f), 1000.f) - 20 : 0;
+    auto scaled = [&](f4_t v, float f) {
+        v *= f;
+        if (SCALED)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(v[i], back);
+        return v;
+    };
     float *const part = p.partials + (int64_t)blockIdx.x * PARTIAL;
 
     if (WK == 1) {
@@ -1012,7 +1096,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         const int row_in_tile = wr * RW + col;
         float *to = pieces > 1 ? part + row_in_tile * DP
                                : p.out + (int64_t)(it.start + token) * p.out_stride + (int64_t)head * dim;
-        const float by = pieces > 1 ? 1.f : l == 0.f ? 0.f : kDown / l;
+        const float by = l == 0.f ? 0.f : 1.f / l;
         const int width = pieces > 1 ? DP : dim;
         if (any_odd) {
 #pragma unroll
@@ -1028,45 +1112,42 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
             for (int j = 0; j < REGS / 4; ++j) {
                 const int d = RW * db + 8 * j + 4 * part_of;
                 const f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
-                if (d < width) *(f4_t *)(to + d) = v * by;
+                if (d < width) *(f4_t *)(to + d) = scaled(v, by);
             }
         if (pieces > 1 && part_of == 0) {
-            const f2_t v = {r, l};
+            const f2_t v = {m, l};
             *(f2_t *)(part + LAYOUT * DP + 2 * row_in_tile) = v;
         }
     } else {
         /* the waves' results meet in LDS */
         if (part_of == 0) {
-            joined[wk][0][col] = r;
+            joined[wk][0][col] = m;
             joined[wk][1][col] = l;
         }
         lds_barrier(); /* tiles are done with, too */
         float top = joined[0][0][col];
 #pragma unroll
         for (int w = 1; w < WK; ++w) top = fmaxf(top, joined[w][0][col]);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) sum += joined[w][1][col] * __builtin_amdgcn_exp2f(joined[w][0][col] - top);
         float *mine = (float *)lds + wk * RW * DP;
-        const float fade = __builtin_amdgcn_exp2f(r - top);
+        const float share = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top) / sum;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int j = 0; j < REGS / 4; ++j) {
                 const int d4 = RW / 4 * db + 2 * j + part_of;
                 const f4_t v = {o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
-                *(f4_t *)(mine + col * DP + ((d4 ^ (col & 7)) << 2)) = v * fade;
+                *(f4_t *)(mine + col * DP + ((d4 ^ (col & 7)) << 2)) = scaled(v, share);
             }
         lds_barrier();
         const int rows = min(it.n * group - it.tile * S::ROWS, S::ROWS);
         for (int e = tid; e < rows * (DP / 4); e += THREADS) {
             const int rr = e / (DP / 4), d4 = e % (DP / 4);
-            float all = joined[0][0][rr], sum = 0.f;
-#pragma unroll
-            for (int w = 1; w < WK; ++w) all = fmaxf(all, joined[w][0][rr]);
             f4_t v = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
-                v += *(const f4_t *)((const float *)lds + w * RW * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
-            }
+            for (int w = 0; w < WK; ++w) v += *(const f4_t *)((const float *)lds + w * RW * DP + rr * DP + ((d4 ^ (rr & 7)) << 2));
             const int tile_row = it.tile * S::ROWS + rr, tk = tile_row / group;
             if (any_odd) {
 #pragma unroll
@@ -1075,11 +1156,15 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
             }
             if (pieces == 1) {
                 float *out = p.out + (int64_t)(it.start + tk) * p.out_stride + (int64_t)(kvh * group + tile_row - tk * group) * dim;
-                v *= sum == 0.f ? 0.f : kDown / sum;
                 if (4 * d4 < dim) *(f4_t *)(out + 4 * d4) = v;
             } else {
                 *(f4_t *)(part + rr * DP + 4 * d4) = v;
                 if (d4 == 0) {
+                    float all = joined[0][0][rr], sum = 0.f;
+#pragma unroll
+                    for (int w = 1; w < WK; ++w) all = fmaxf(all, joined[w][0][rr]);
+#pragma unroll
+                    for (int w = 0; w < WK; ++w) sum += joined[w][1][rr] * __builtin_amdgcn_exp2f(joined[w][0][rr] - all);
                     const f2_t st = {all, sum};
                     *(f2_t *)(part + LAYOUT * DP + 2 * rr) = st;
                 }
@@ -1128,11 +1213,13 @@ void attention_kernel(AttnParams p)
 }
 
 /* Joins the pieces of rows whose keys were cut, in their order within each of
- * GROUPS groups of threads and then in the groups' order. A second kernel:
+ * GROUPS groups of threads and then in the groups' order: each is the average of
+ * its values, with its weights' reference and sum, and the join averages those
+ * by the sums. A second kernel:
  * joined by the last workgroup of a tile, the 128 pieces of one row tile at
  * 32749 keys took 17 us of one compute unit. */
 template <int DP, int ROWS, int GROUPS>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int slices, float down)
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int slices)
 {
     constexpr int D4 = DP / 4, EACH = 256 / (D4 * GROUPS); /* rows of a workgroup */
     constexpr int AT_ONCE = GROUPS > 1 ? 8 : 16;
@@ -1170,17 +1257,20 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
                 float top = all;
 #pragma unroll
                 for (int i = 0; i < N; ++i) top = fmaxf(top, st[i][0]);
-                const float fade = __builtin_amdgcn_exp2f(all - top);
+                const float before = sum * __builtin_amdgcn_exp2f(all - top);
+                float g[N];
                 all = top;
-                sum *= fade;
-                v *= fade;
+                sum = before;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    g[i] = i0 + i < i_end ? st[i][1] * __builtin_amdgcn_exp2f(st[i][0] - all) : 0.f;
+                    sum += g[i];
+                }
+                const float by = sum == 0.f ? 0.f : 1.f / sum;
+                v *= before * by;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (i0 + i < i_end) {
-                        const float f = __builtin_amdgcn_exp2f(st[i][0] - all);
-                        sum = fmaf(st[i][1], f, sum);
-                        v += x[i] * f;
-                    }
+                    if (i0 + i < i_end) v += x[i] * (g[i] * by);
             };
             int i0 = set * mine;
             for (; i_end - i0 > 4; i0 += AT_ONCE) take(std::integral_constant<int, AT_ONCE>(), i0);
@@ -1193,19 +1283,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
             float top = states[0][each][0];
 #pragma unroll
             for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, states[i][each][0]);
-            v = f4_t{0, 0, 0, 0};
+            float g[GROUPS];
             sum = 0.f;
 #pragma unroll
             for (int i = 0; i < GROUPS; ++i) {
-                const float f = __builtin_amdgcn_exp2f(states[i][each][0] - top);
-                sum = fmaf(states[i][each][1], f, sum);
-                v += sums[i][each][d4] * f;
+                g[i] = states[i][each][1] * __builtin_amdgcn_exp2f(states[i][each][0] - top);
+                sum += g[i];
             }
+            const float by = sum == 0.f ? 0.f : 1.f / sum;
+            v = f4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) v += sums[i][each][d4] * (g[i] * by);
             __syncthreads();
         }
         if (real && set == 0 && 4 * d4 < a.dim) {
             float *out = p.out + (int64_t)(j.start + token) * p.out_stride + (int64_t)(kvh * group + row - token * group) * a.dim;
-            *(f4_t *)(out + 4 * d4) = v * (sum == 0.f ? 0.f : down / sum);
+            *(f4_t *)(out + 4 * d4) = v;
         }
     }
 }
@@ -1290,14 +1383,14 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     return plan;
 }
 
-template <int DP, int ROWS, int GROUPS> static void launch_join(const AttnParams &p, const AttnPlan &plan, float down, hipStream_t s)
+template <int DP, int ROWS, int GROUPS> static void launch_join(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     constexpr int EACH = 256 / (DP / 4 * GROUPS); /* rows of a workgroup */
     /* workgroups of a tile for the rows that a sequence has on average */
     const int64_t each = ((int64_t)p.t.tokens * (p.t.heads / p.t.kv_heads) + p.t.count - 1) / p.t.count;
     const int slices = (int)(((each < ROWS ? each : ROWS) + EACH - 1) / EACH);
     const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * slices);
-    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices, down);
+    attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices);
 }
 
 template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
@@ -1306,12 +1399,11 @@ template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(con
     if (plan.lists) attention_list_kernel<S::ROWS, S::KT * WK><<<1, 1024, 0, s>>>(p);
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
     if (plan.target == 0) return;
-    const float down = TYPE == QMV_KV_F16 ? 1.f : 9.5367431640625e-07f;
     /* Groups of threads where a tile has many pieces (the tiles counted here are an
      * upper bound): 4 tokens over 32000 keys 31 us, 48 with one group; 64 sequences
      * of 1000 keys 34 with groups, 32 with one. */
-    if (plan.target >= 8 * plan.tiles * p.t.kv_heads) launch_join<DP, S::ROWS, 8>(p, plan, down, s);
-    else launch_join<DP, S::ROWS, 1>(p, plan, down, s);
+    if (plan.target >= 8 * plan.tiles * p.t.kv_heads) launch_join<DP, S::ROWS, 8>(p, plan, s);
+    else launch_join<DP, S::ROWS, 1>(p, plan, s);
 }
 
 template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
