@@ -460,9 +460,12 @@ int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride,
  * value below 2^-60 of a row's largest. The weights' sum is of fp32. Where the
  * values of a row's blocks of 16 tokens differ by more than 2^10 in size, the
  * products take about twice the time.
- * A key that is not finite
- * makes the rows that attend it NaN, a value the elements that sum it not
- * finite; neither reaches other rows.
+ * A key that is not finite makes the rows that attend it NaN, except that
+ * infinite elements of f16 and bf16 may give a score of minus infinity, which
+ * has no weight; a row whose scores are all minus infinity is NaN. A value that
+ * is not finite makes the elements that sum it not finite. Neither reaches other
+ * rows. Scores count times log2(e), so from 2.3e38 on as infinite, and so does
+ * scale times an element of q.
  * The work of few rows is cut along the length and joined in a fixed order: the
  * same call gives the same bits. What the pieces pass to each other, and the
  * limbs of long prompts, are in a workspace of the stream, so a capture needs

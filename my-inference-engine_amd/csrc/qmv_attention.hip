@@ -353,8 +353,8 @@ struct AttnLists {
 
 /* What the pieces' join has to know of a row tile whose keys are cut. */
 struct AttnJoin {
-    int start, n, tile; /* as in AttnItem */
-    int pieces;         /* 0: not cut */
+    int start, n, first, tile; /* as in AttnItem */
+    int pieces;                /* 0: not cut */
     int item, apart;    /* the first piece's number, and what the next ones' are apart */
 };
 
@@ -728,7 +728,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
     const int pieces = max((int)(((int64_t)keys + it.chunk - 1) / it.chunk), 1);
     if (it.split >= pieces) return;
     if (p.target && kvh == 0 && it.split == 0 && tid == 0)
-        p.joins[1 + it.tile_at] = AttnJoin{it.start, it.n, it.tile, pieces > 1 ? pieces : 0, item, it.tiles};
+        p.joins[1 + it.tile_at] = AttnJoin{it.start, it.n, it.first, it.tile, pieces > 1 ? pieces : 0, item, it.tiles};
     const int begin = it.split * it.chunk, end = min((int64_t)keys, (int64_t)begin + it.chunk);
     const int unmasked = it.first + it.tile * S::ROWS / group; /* every row attends keys up to here */
 
@@ -1080,6 +1080,9 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         }
     }
     l = sum_lanes<RW>(l);
+    /* A row without weights: zeros if it attends nothing; if all its scores are
+     * minus infinity NaN, as 0 / 0 is (of pieces their join says so). */
+    const float nothing = pieces == 1 && pos >= 0 ? NAN : 0.f;
     /* O to the sums themselves, together with the factor 1 / l */
     const int back = SCALED ? (int)fminf(fmaxf(rm, -1000.f), 1000.f) - 20 : 0;
     auto scaled = [&](f4_t v, float f) {
@@ -1096,7 +1099,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         const int row_in_tile = wr * RW + col;
         float *to = pieces > 1 ? part + row_in_tile * DP
                                : p.out + (int64_t)(it.start + token) * p.out_stride + (int64_t)head * dim;
-        const float by = l == 0.f ? 0.f : 1.f / l;
+        const float by = l == 0.f ? nothing : 1.f / l;
         const int width = pieces > 1 ? DP : dim;
         if (any_odd) {
 #pragma unroll
@@ -1132,7 +1135,7 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
 #pragma unroll
         for (int w = 0; w < WK; ++w) sum += joined[w][1][col] * __builtin_amdgcn_exp2f(joined[w][0][col] - top);
         float *mine = (float *)lds + wk * RW * DP;
-        const float share = sum == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - top) / sum;
+        const float share = sum == 0.f ? nothing : __builtin_amdgcn_exp2f(m - top) / sum;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -1298,7 +1301,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
         }
         if (real && set == 0 && 4 * d4 < a.dim) {
             float *out = p.out + (int64_t)(j.start + token) * p.out_stride + (int64_t)(kvh * group + row - token * group) * a.dim;
-            *(f4_t *)(out + 4 * d4) = v;
+            const float nothing = sum == 0.f && j.first + token >= 0 ? NAN : 0.f; /* as in attend_piece; added, as a branch took 1 us more */
+            *(f4_t *)(out + 4 * d4) = v + nothing;
         }
     }
 }

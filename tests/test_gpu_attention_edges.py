@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import _attention as A
-from test_gpu_attention import _prompt, _rand, _rope_bound, hip  # noqa: F401
+from test_gpu_attention import _paged, _paged_case, _prompt, _rand, _rope_bound, hip  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,39 @@ def test_scores_far_below_zero(qmv, hip):  # noqa: F811
         for i in range(n):
             ref, size = v[:i + 1, 0].astype(np.float64).mean(0), np.abs(v[:i + 1, 0]).astype(np.float64).mean(0)
             assert (np.abs(o[i] - ref) <= (2 * 2.0 ** -22 + 2 * (i + 1) * 2.0 ** -23 + 2.0 ** -22) * size).all(), (n, dim, i)
+
+
+@pytest.mark.parametrize("t", A.TYPES, ids=lambda t: A.NAMES[t])
+@pytest.mark.parametrize("new,length", [([1, 20, 1], [40, 60, 33]), ([1, 2], [2000, 1500]), ([45], [2200])])
+def test_infinite_keys(qmv, hip, t, new, length):  # noqa: F811
+    """Rows whose every score is minus infinity are NaN, like 0 / 0, not zeros;
+    one infinite key gives NaN, or has no weight; other rows see none of it. The
+    queries' element that meets the infinities is above zero."""
+    heads, kv_heads, dim = 7, 1, 128
+    b, q, keys, values, _ = _paged_case(qmv, hip, new, length, heads, kv_heads, dim, t, 16, seed=35)
+    q[..., 2] = 1 + 0.137 * np.arange(heads)  # whose limbs are of one sign for some heads, and not for others
+    odd = [k.copy() for k in keys]
+    odd[0][:, 0, 2] = -np.inf
+    last = len(new) - 1
+    if last:
+        odd[last][3, 0, 2] = -np.inf
+    o, ok = _paged(qmv, hip, b, q, A.Cache(qmv, hip, b, odd, values, t), dim ** -0.5)
+    assert ok == 1
+    assert np.isnan(o[:new[0]]).all()
+    for s in range(1, len(new)):
+        a, n = int(b.starts[s]), new[s]
+        keep = np.arange(length[s]) != (3 if s == last else -1)
+        ref, bound = A.attention64(q[a:a + n], keys[s][keep], values[s][keep], dim ** -0.5, [p - (s == last) for p in b.positions(s)])
+        for i in range(n):
+            for h in range(heads):
+                dropped = (np.abs(o[a + i, h] - ref[i, h]) <= bound[i, h]).all()
+                assert dropped or (s == last and np.isnan(o[a + i, h]).all()), (s, i, h)
+
+
+def test_prompt_scores_of_minus_infinity(qmv, hip):  # noqa: F811
+    """As above for finite keys whose scores are below the lowest number."""
+    for n in (5, 700, 1100):
+        q, k = np.zeros((n, 4, 128), np.float32), np.zeros((n, 2, 128), np.float32)
+        q[..., 3], k[..., 3] = 3e19, -3e19
+        v = _rand(np.random.default_rng(42), n, 2, 128)
+        assert np.isnan(_prompt(qmv, hip, [n], 4, 2, 128, q, k, v, 1.0)).all()
