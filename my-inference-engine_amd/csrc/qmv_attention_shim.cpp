@@ -7,15 +7,9 @@
 
 #include <climits>
 #include <cmath>
-#include <cstdarg>
 #include <cstdint>
-#include <cstdio>
 #include <exception>
-#include <map>
-#include <memory>
 #include <mutex>
-#include <utility>
-#include <vector>
 
 #include "qmv_hip.h"
 #include "qmv_kernels.h"
@@ -25,34 +19,8 @@
 
 namespace {
 
-void set_error(const char *fmt, ...)
-{
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    qmv::shim_error(buf);
-}
-
-bool hip_ok(hipError_t e, const char *what)
-{
-    if (e == hipSuccess) return true;
-    set_error("%s failed: %s", what, hipGetErrorString(e));
-    return false;
-}
-
-#define HIP_TRY(expr)                         \
-    do {                                      \
-        if (!hip_ok((expr), #expr)) return 0; \
-    } while (0)
-
-/* Byte ranges that share a byte. */
-bool overlap(const void *a, size_t abytes, const void *b, size_t bbytes)
-{
-    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-    return a0 < b0 + bbytes && b0 < a0 + abytes;
-}
+using qmv::overlap;
+using qmv::set_error;
 
 /* Bytes of `rows` rows of `width` floats that are `stride` apart. */
 size_t rows_bytes(int rows, int64_t stride, int64_t width)
@@ -176,48 +144,6 @@ qmv::AttnTokens attn_tokens(const QmvSequences &q, int tokens, int heads, int kv
     return t;
 }
 
-/* What the pieces of a stream's calls leave for their join. The buffer only
- * grows, and one that is replaced is kept: a graph captured earlier on the
- * stream may still use it. */
-struct Workspace {
-    unsigned char *data = nullptr;
-    size_t cap = 0;
-    std::vector<void *> retired;
-    std::mutex mu;
-};
-
-std::mutex g_workspaces_mu;
-std::map<std::pair<int, const void *>, std::unique_ptr<Workspace>> g_workspaces;
-
-/* Threads share the handle of the per-thread stream and not the stream. */
-thread_local char t_stream;
-
-Workspace &workspace_for(int device, hipStream_t stream)
-{
-    std::lock_guard<std::mutex> lock(g_workspaces_mu);
-    auto &slot = g_workspaces[{device, stream == hipStreamPerThread ? (const void *)&t_stream : (const void *)stream}];
-    if (!slot) slot.reset(new Workspace());
-    return *slot;
-}
-
-/* The workspace grown to `bytes`, its mutex held. */
-int workspace_reserve(Workspace &ws, hipStream_t stream, size_t bytes)
-{
-    if (bytes <= ws.cap) return 1;
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
-        set_error("workspace must grow during stream capture; run the call once before capturing");
-        return 0;
-    }
-    const size_t n = bytes + bytes / 2;
-    void *buf = nullptr;
-    HIP_TRY(qmv::shim_malloc(&buf, n));
-    if (ws.data) ws.retired.push_back(ws.data);
-    ws.data = (unsigned char *)buf;
-    ws.cap = n;
-    return 1;
-}
-
 int attend(qmv::AttnParams &p, int type, hipStream_t stream)
 try {
     const int device = qmv::shim_device();
@@ -227,12 +153,11 @@ try {
         set_error("too many tokens and heads for one call");
         return 0;
     }
-    Workspace &ws = workspace_for(device, stream);
-    std::lock_guard<std::mutex> lock(ws.mu);
+    unsigned char *at = nullptr;
+    std::unique_lock<std::mutex> lock; /* until the launches are made */
     const size_t partial_bytes = plan.partials * sizeof(float), joins = (plan.joins + 15) / 16 * 16;
     const size_t counts = (size_t)p.t.count * sizeof(int2);
-    if (!workspace_reserve(ws, stream, plan.image_bytes + partial_bytes + joins + plan.lists)) return 0;
-    unsigned char *at = ws.data;
+    if (!qmv::shim_scratch(device, stream, plan.image_bytes + partial_bytes + joins + plan.lists, &at, &lock)) return 0;
     p.target = plan.target;
     p.alike = plan.alike;
     p.least = plan.least;

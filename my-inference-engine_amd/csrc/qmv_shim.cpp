@@ -53,11 +53,11 @@ struct QmvDeviceTensor {
     uint8_t *rowmajor; /* row-major copy (Q4_K: the GGUF bytes; Q6_K: planes), else null */
 };
 
-namespace {
-
 /* ---- errors ----------------------------------------------------------------- */
 
-thread_local std::string t_error;
+namespace qmv {
+
+static thread_local std::string t_error;
 
 void set_error(const char *fmt, ...)
 {
@@ -76,10 +76,19 @@ bool hip_ok(hipError_t e, const char *what)
     return false;
 }
 
-#define HIP_TRY(expr)                         \
-    do {                                      \
-        if (!hip_ok((expr), #expr)) return 0; \
-    } while (0)
+bool overlap(const void *a, size_t abytes, const void *b, size_t bbytes)
+{
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    return a0 < b0 + bbytes && b0 < a0 + abytes;
+}
+
+} // namespace qmv
+
+namespace {
+
+using qmv::hip_ok;
+using qmv::overlap;
+using qmv::set_error;
 
 std::atomic<int> g_device{0};
 std::atomic<int> g_fail_next{0};
@@ -102,13 +111,6 @@ hipError_t counted_host_malloc(void **p, size_t bytes)
 }
 
 /* ---- validation (src/quantized_matvec.cpp:93-149, :168-191) ------------------ */
-
-/* Byte ranges that share a byte. */
-bool overlap(const void *a, size_t abytes, const void *b, size_t bbytes)
-{
-    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
-    return a0 < b0 + bbytes && b0 < a0 + abytes;
-}
 
 struct Shape {
     QmvGeometry geo;
@@ -181,6 +183,9 @@ struct Workspace {
     uint64_t *fused_cand = nullptr;  /* fused argmax: tile and group candidates */
     unsigned *fused_count = nullptr; /* fused argmax: arrival counts, zero between launches */
     size_t fused_cap = 0;            /* tiles */
+    unsigned char *scratch = nullptr; /* attention: the pieces' results, limbs, lists */
+    size_t scratch_cap = 0;
+    uint64_t thread = 0; /* of a per-thread stream: whose */
     /* Buffers replaced by a larger one. They are never freed: a graph
      * captured earlier on this stream still launches kernels that use them
      * (every launch leaves its counters at zero, so such replays stay
@@ -190,17 +195,25 @@ struct Workspace {
     std::mutex mu;
 };
 
+/* Not while the stream is captured: the allocation would not be part of the
+ * graph. */
+int workspace_may_grow(hipStream_t stream)
+{
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
+        set_error("workspace must grow during stream capture; run the call once before capturing");
+        return 0;
+    }
+    return 1;
+}
+
 /* Grow the workspace; waits for work already queued on the stream. New
  * counters are zeroed on the stream the kernels run on (never inside a graph
  * capture: growth is refused there), so every launch finds them zero. */
 int workspace_reserve(Workspace &ws, hipStream_t stream, size_t partials, size_t counters)
 {
     if (partials <= ws.partial_cap && counters <= ws.counter_cap) return 1;
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
-        set_error("workspace must grow during stream capture; run the call once before capturing");
-        return 0;
-    }
+    if (!workspace_may_grow(stream)) return 0;
     HIP_TRY(hipStreamSynchronize(stream));
     if (partials > ws.partial_cap) {
         const size_t n = partials + partials / 2 + 4096;
@@ -230,11 +243,7 @@ constexpr int kArgBlocks = 512;
 int workspace_fused_argmax(Workspace &ws, hipStream_t stream, size_t tiles)
 {
     if (tiles <= ws.fused_cap) return 1;
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone) {
-        set_error("workspace must grow during stream capture; run the call once before capturing");
-        return 0;
-    }
+    if (!workspace_may_grow(stream)) return 0;
     HIP_TRY(hipStreamSynchronize(stream));
     const size_t n = tiles + tiles / 2 + 256;
     uint64_t *cand = nullptr;
@@ -265,13 +274,31 @@ int workspace_argmax(Workspace &ws)
 }
 
 std::mutex g_ws_mu;
-std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>> g_workspaces;
+std::map<std::pair<int, const void *>, std::unique_ptr<Workspace>> g_workspaces;
+std::vector<std::unique_ptr<Workspace>> g_left_workspaces; /* in use when a thread ended */
+
+/* Threads share the handle of the per-thread stream and not the stream: each
+ * has a workspace of its own there, by the address of a variable of its own. A
+ * later thread may get the address of one that has ended, and with it the
+ * workspace, once the work that used it is done. */
+std::atomic<uint64_t> g_threads{0};
+thread_local uint64_t t_thread = 0;
 
 Workspace &workspace_for(int device, hipStream_t stream)
 {
+    const bool own = stream == hipStreamPerThread;
     std::lock_guard<std::mutex> lock(g_ws_mu);
-    auto &slot = g_workspaces[{device, stream}];
+    auto &slot = g_workspaces[{device, own ? (const void *)&t_thread : (const void *)stream}];
+    if (own) {
+        if (t_thread == 0) t_thread = ++g_threads;
+        if (slot && slot->thread != t_thread) {
+            hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+            const bool captured = hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone;
+            if (captured || hipDeviceSynchronize() != hipSuccess) g_left_workspaces.push_back(std::move(slot));
+        }
+    }
     if (!slot) slot.reset(new Workspace());
+    if (own) slot->thread = t_thread;
     return *slot;
 }
 
@@ -2314,28 +2341,31 @@ QMV_API int qmv_device_dequantize_f32(qmv_device_tensor t, int first_row, int ro
 
 /* ---- what the attention entry points share with these (qmv_shim.h) ---------- */
 
-namespace qmv {
-
-void shim_error(const char *text)
-{
-    t_error = text;
-}
-
-int shim_device()
+int qmv::shim_device()
 {
     return g_device.load();
 }
 
-hipError_t shim_malloc(void **p, size_t bytes)
+int qmv::shim_scratch(int device, hipStream_t stream, size_t bytes, unsigned char **data, std::unique_lock<std::mutex> *lock)
 {
-    return counted_malloc(p, bytes);
+    Workspace &ws = workspace_for(device, stream);
+    *lock = std::unique_lock<std::mutex>(ws.mu);
+    if (bytes > ws.scratch_cap) {
+        if (!workspace_may_grow(stream)) return 0;
+        const size_t n = bytes + bytes / 2;
+        void *buf = nullptr;
+        HIP_TRY(counted_malloc(&buf, n));
+        if (ws.scratch) ws.retired.push_back(ws.scratch);
+        ws.scratch = (unsigned char *)buf;
+        ws.scratch_cap = n;
+    }
+    *data = ws.scratch;
+    return 1;
 }
-
-} // namespace qmv
 
 QMV_API const char *qmv_last_error(void)
 {
-    return t_error.c_str();
+    return qmv::t_error.c_str();
 }
 
 QMV_API int qmv_set_device(int ordinal)

@@ -1,9 +1,12 @@
 """Calls of the operators between the projections that the documentation allows
 at its edges, against 64 bits."""
+import threading
+
 import numpy as np
 import pytest
 
 import _attention as A
+import _blocks as B
 from test_gpu_attention import _paged, _paged_case, _prompt, _rand, _rope_bound, hip  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +90,49 @@ def test_prompt_scores_of_minus_infinity(qmv, hip):  # noqa: F811
         q[..., 3], k[..., 3] = 3e19, -3e19
         v = _rand(np.random.default_rng(42), n, 2, 128)
         assert np.isnan(_prompt(qmv, hip, [n], 4, 2, 128, q, k, v, 1.0)).all()
+
+
+# ---- workspaces ---------------------------------------------------------------------------
+
+PER_THREAD = 2  # hipStreamPerThread
+
+
+def test_threads_on_per_thread_streams(qmv, hip):  # noqa: F811
+    """Threads that name their own stream by the one handle for it do not share
+    a workspace: attention in pieces and a product split along K, in two threads
+    at once, then in short-lived threads one after the other (whose variables
+    take each other's places). Every result has the bits of a call by itself."""
+    cases = [_paged_case(qmv, hip, [1, 2], [1900, 900 + 300 * i], 14, 2, 64, A.F16, 16, seed=50 + i) for i in range(2)]
+    rows, cols = 64, 18944
+    raws = [qmv.synth_tensor(B.Q4_K, rows, cols, seed=60 + i) for i in range(2)]
+    weights = [qmv.DeviceTensor(qmv.make_view(raw, B.Q4_K, rows, cols)) for raw in raws]
+    work, expected, failures = [], [], []
+    for i, (b, q, keys, values, cache) in enumerate(cases):
+        x = hip.DeviceBuffer.from_array(np.random.default_rng(i).standard_normal(4 * cols).astype(np.float32))
+        work.append((hip.DeviceBuffer.from_array(q), hip.DeviceBuffer(q.nbytes), b.upload(qmv, hip), cache, x, hip.DeviceBuffer(16 * rows)))
+
+    def once(i, stream):
+        dq, do, seq, cache, x, y = work[i]
+        qmv.device_attention_paged(dq.ptr, 3, 14, 0.125, seq, cache.c, do.ptr, stream)
+        qmv.device_matvec_group([weights[i]], x.ptr, 4, [y.ptr], stream)
+        hip.check(hip.rt().hipStreamSynchronize(stream))
+        return do.to_array(np.uint32, do.nbytes // 4), y.to_array(np.uint32, 4 * rows)
+
+    def run(i, times):
+        try:
+            for _ in range(times):
+                if not all(np.array_equal(a, e) for a, e in zip(once(i, PER_THREAD), expected[i])):
+                    failures.append(i)
+        except Exception as e:  # noqa: BLE001
+            failures.append(repr(e))
+
+    for i in range(2):
+        expected.append(once(i, 0))
+    for groups, times in (([[0, 1]], 30), ([[k % 2] for k in range(8)], 2)):
+        for group in groups:
+            threads = [threading.Thread(target=run, args=(i, times)) for i in group]
+            [t.start() for t in threads]
+            [t.join() for t in threads]
+    assert failures == []
+    for w in weights:
+        w.close()
