@@ -73,6 +73,7 @@ bool hip_ok(hipError_t e, const char *what)
 {
     if (e == hipSuccess) return true;
     set_error("%s failed: %s", what, hipGetErrorString(e));
+    (void)hipGetLastError(); /* reported: not again by the next launch's check */
     return false;
 }
 

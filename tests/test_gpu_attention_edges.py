@@ -7,6 +7,7 @@ import pytest
 
 import _attention as A
 import _blocks as B
+from _attention_plan import plan
 from test_gpu_attention import _paged, _paged_case, _prompt, _rand, _rope_bound, hip  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -136,3 +137,18 @@ def test_threads_on_per_thread_streams(qmv, hip):  # noqa: F811
     assert failures == []
     for w in weights:
         w.close()
+
+
+def test_a_refused_allocation_leaves_no_error(qmv, hip):  # noqa: F811
+    """A call whose workspace the card cannot hold (the images of 2^22 - 64 tokens of
+    256 heads, 1.1 TB) is refused before any launch, so that its addresses are
+    never read; the next call of the thread is not told of it."""
+    tokens, heads = (1 << 22) - 64, 256
+    assert plan(tokens, heads, heads, 128, 1).images * (64 * 128 * 8 + 256) > 1 << 40
+    starts = hip.DeviceBuffer.from_array(np.array([0, tokens], np.int32))
+    with pytest.raises(qmv.QmvError, match="memory"):
+        qmv.device_attention_prompt(1 << 44, 2 << 44, 3 << 44, tokens, heads, heads, 128, 0.1, qmv.make_sequences(starts.ptr, 1), 4 << 44)
+    rng = np.random.default_rng(44)
+    q, k, v = _rand(rng, 9, 2, 64), _rand(rng, 9, 1, 64), _rand(rng, 9, 1, 64)
+    ref, bound = A.attention64(q, k, v, 0.125, range(9))
+    assert (np.abs(_prompt(qmv, hip, [9], 2, 1, 64, q, k, v, 0.125) - ref) <= bound).all()
