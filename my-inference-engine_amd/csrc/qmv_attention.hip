@@ -1387,7 +1387,7 @@ AttnPlan plan_attention(const AttnTokens &t, int type)
     return plan;
 }
 
-template <int DP, int ROWS, int GROUPS> static void launch_join(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+template <int DP, int ROWS, int GROUPS> static hipError_t launch_join(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     constexpr int EACH = 256 / (DP / 4 * GROUPS); /* rows of a workgroup */
     /* workgroups of a tile for the rows that a sequence has on average */
@@ -1395,51 +1395,54 @@ template <int DP, int ROWS, int GROUPS> static void launch_join(const AttnParams
     const int slices = (int)(((each < ROWS ? each : ROWS) + EACH - 1) / EACH);
     const unsigned grid = (unsigned)(plan.tiles * p.t.kv_heads * slices);
     attention_join_kernel<DP, ROWS, GROUPS><<<dim3(grid), 256, 0, s>>>(p, slices);
+    return hipGetLastError();
 }
 
-template <int TYPE, int DP, int RW, int WR, int WK> static void launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+/* Each kernel reads what the one before it wrote, and is launched only after it
+ * has been. */
+template <int TYPE, int DP, int RW, int WR, int WK> static hipError_t launch_shape(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     using S = AttnShape<TYPE, DP, RW, WR, WK>;
-    if (plan.lists) attention_list_kernel<S::ROWS, S::KT * WK><<<1, 1024, 0, s>>>(p);
+    if (plan.lists) {
+        attention_list_kernel<S::ROWS, S::KT * WK><<<1, 1024, 0, s>>>(p);
+        if (const hipError_t e = hipGetLastError()) return e;
+    }
     attention_kernel<TYPE, DP, RW, WR, WK><<<dim3((unsigned)plan.grid), 64 * WR * WK, 0, s>>>(p);
-    if (plan.target == 0) return;
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || plan.target == 0) return e;
     /* Groups of threads where a tile has many pieces (the tiles counted here are an
      * upper bound): 4 tokens over 32000 keys 31 us, 48 with one group; 64 sequences
      * of 1000 keys 34 with groups, 32 with one. */
-    if (plan.target >= 8 * plan.tiles * p.t.kv_heads) launch_join<DP, S::ROWS, 8>(p, plan, s);
-    else launch_join<DP, S::ROWS, 1>(p, plan, s);
+    if (plan.target >= 8 * plan.tiles * p.t.kv_heads) return launch_join<DP, S::ROWS, 8>(p, plan, s);
+    return launch_join<DP, S::ROWS, 1>(p, plan, s);
 }
 
-template <int TYPE, int DP> static void launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+template <int TYPE, int DP> static hipError_t launch_rows(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
-    if (plan.rows == 16) launch_shape<TYPE, DP, 16, 1, 4>(p, plan, s);
-    else if (plan.rows == 32) launch_shape<TYPE, DP, 32, 1, 4>(p, plan, s);
-    else if (plan.rows == 128) launch_shape<TYPE, DP, 32, 4, 1>(p, plan, s);
-    else launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
+    if (plan.rows == 16) return launch_shape<TYPE, DP, 16, 1, 4>(p, plan, s);
+    if (plan.rows == 32) return launch_shape<TYPE, DP, 32, 1, 4>(p, plan, s);
+    if (plan.rows == 128) return launch_shape<TYPE, DP, 32, 4, 1>(p, plan, s);
+    return launch_shape<TYPE, DP, 32, 8, 1>(p, plan, s);
 }
 
 /* A prompt's rows of fp32, through images of their tiles. */
-template <int DP> static void launch_images(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+template <int DP> static hipError_t launch_images(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
     attention_image_kernel<DP><<<dim3((unsigned)plan.images), 256, 0, s>>>(p);
-    launch_shape<QMV_KV_IMAGE, DP, 32, 8, 1>(p, plan, s);
+    if (const hipError_t e = hipGetLastError()) return e;
+    return launch_shape<QMV_KV_IMAGE, DP, 32, 8, 1>(p, plan, s);
 }
 
-template <int TYPE> static void launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
+template <int TYPE> static hipError_t launch_dim(const AttnParams &p, const AttnPlan &plan, hipStream_t s)
 {
-    if (p.t.dim <= 64) launch_rows<TYPE, 64>(p, plan, s);
-    else launch_rows<TYPE, 128>(p, plan, s);
+    return p.t.dim <= 64 ? launch_rows<TYPE, 64>(p, plan, s) : launch_rows<TYPE, 128>(p, plan, s);
 }
 
 hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s)
 {
-    if (plan.images) {
-        if (p.t.dim <= 64) launch_images<64>(p, plan, s);
-        else launch_images<128>(p, plan, s);
-    } else if (type == QMV_KV_F32) launch_dim<QMV_KV_F32>(p, plan, s);
-    else if (type == QMV_KV_F16) launch_dim<QMV_KV_F16>(p, plan, s);
-    else launch_dim<QMV_KV_BF16>(p, plan, s);
-    return hipGetLastError();
+    if (plan.images) return p.t.dim <= 64 ? launch_images<64>(p, plan, s) : launch_images<128>(p, plan, s);
+    if (type == QMV_KV_F32) return launch_dim<QMV_KV_F32>(p, plan, s);
+    return type == QMV_KV_F16 ? launch_dim<QMV_KV_F16>(p, plan, s) : launch_dim<QMV_KV_BF16>(p, plan, s);
 }
 
 /* A workgroup per token: the pairs' sines once in LDS, then all heads. Bound by

@@ -56,7 +56,7 @@ bool heads_ok(int tokens, int q_heads, int kv_heads, int head_dim)
         set_error("invalid token or head counts (%d tokens, %d and %d heads)", tokens, q_heads, kv_heads);
         return false;
     }
-    if ((int64_t)tokens * q_heads > INT_MAX / 2) {
+    if ((int64_t)tokens * q_heads > 1 << 30) {
         set_error("more than 2^30 rows of tokens and heads");
         return false;
     }
@@ -146,13 +146,14 @@ qmv::AttnTokens attn_tokens(const QmvSequences &q, int tokens, int heads, int kv
 
 int attend(qmv::AttnParams &p, int type, hipStream_t stream)
 try {
-    const int device = qmv::shim_device();
-    HIP_TRY(hipSetDevice(device));
     const qmv::AttnPlan plan = qmv::plan_attention(p.t, type);
-    if (plan.grid > INT_MAX || plan.images > INT_MAX) {
-        set_error("too many tokens and heads for one call");
+    /* a launch has less than 2^32 threads */
+    if (plan.grid * qmv::attention_threads(plan) > UINT32_MAX || plan.images * 256 > UINT32_MAX) {
+        set_error("too many tokens, sequences and heads for one call");
         return 0;
     }
+    const int device = qmv::shim_device();
+    HIP_TRY(hipSetDevice(device));
     unsigned char *at = nullptr;
     std::unique_lock<std::mutex> lock; /* until the launches are made */
     const size_t partial_bytes = plan.partials * sizeof(float), joins = (plan.joins + 15) / 16 * 16;

@@ -218,6 +218,8 @@ struct RopeParams {
 #define QMV_KV_BF16 2
 #define QMV_KV_IMAGE 3
 AttnPlan plan_attention(const AttnTokens &t, int type);
+/* Threads of a workgroup: 4 waves, at 256 rows 8. */
+inline int attention_threads(const AttnPlan &plan) { return plan.rows == 256 ? 512 : 256; }
 hipError_t launch_attention(const AttnParams &p, const AttnPlan &plan, int type, hipStream_t s);
 hipError_t launch_rope(const RopeParams &p, int type, hipStream_t s);
 
