@@ -392,9 +392,11 @@ typedef struct QmvPagedCache {
 /*
  * Rotary embedding of the new tokens' queries and keys
  * (src/transformer_ops.cpp:43) and the write of keys and values into the cache,
- * what the decode step does after the q/k/v projections. Token t's heads are rows of head_dim floats from d_q + t * q_stride,
- * d_k + t * k_stride and d_v + t * v_stride (a stride of 0: the heads alone);
- * d_q_out and d_k_out have the strides of d_q and d_k and may be them. Pair i <
+ * what the decode step does after the q/k/v projections. Token t's heads are
+ * rows of head_dim floats from d_q + t * q_stride, d_k + t * k_stride and d_v + t
+ * * v_stride (a stride of 0: the heads alone); d_q_out and d_k_out have the
+ * strides of d_q and d_k and may be them. Other than that an output shares no
+ * floats with any of the rows, which may lie side by side in one buffer. Pair i <
  * rotary_dims / 2 of a head at position p turns by the angle p *
  * d_frequencies[i], a product in 64 bits: (x, y) becomes (x cos - y sin, x sin
  * + y cos) with x, y the elements i and i + rotary_dims / 2, or 2 i and 2 i + 1

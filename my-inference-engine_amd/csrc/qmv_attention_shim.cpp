@@ -10,6 +10,7 @@
 #include <cstdint>
 #include <exception>
 #include <mutex>
+#include <numeric>
 
 #include "qmv_hip.h"
 #include "qmv_kernels.h"
@@ -26,6 +27,17 @@ using qmv::set_error;
 size_t rows_bytes(int rows, int64_t stride, int64_t width)
 {
     return ((size_t)(rows - 1) * (size_t)stride + (size_t)width) * sizeof(float);
+}
+
+/* Whether `rows` rows of wa floats, sa apart, and of wb floats, sb apart, share
+ * any: two rows lie the difference of the first ones and a multiple of the
+ * strides' common divisor apart. (Of unlike strides rows may be said to meet that
+ * are too few to.) */
+bool rows_meet(const float *a, int64_t sa, int64_t wa, const float *b, int64_t sb, int64_t wb, int rows)
+{
+    if (!overlap(a, rows_bytes(rows, sa, wa), b, rows_bytes(rows, sb, wb))) return false;
+    const int64_t g = std::gcd(sa, sb), apart = ((int64_t)((uintptr_t)b - (uintptr_t)a) / 4 % g + g) % g;
+    return apart < wa || apart + wb > g;
 }
 
 bool aligned16(const void *p)
@@ -213,24 +225,28 @@ QMV_API int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q
         }
     }
     /* Heads of rows may lie between those of others (one buffer for q, k and
-     * v): each output may share bytes with rows only as its own input does. */
-    const size_t qb = rows_bytes(tokens, q_stride, (int64_t)q_heads * head_dim);
-    const size_t kb = rows_bytes(tokens, k_stride, (int64_t)kv_heads * head_dim);
-    const size_t vb = cache != nullptr ? rows_bytes(tokens, v_stride, (int64_t)kv_heads * head_dim) : 0;
-    const bool q_apart = d_q_out == d_q || !overlap(d_q_out, qb, d_q, qb);
-    const bool k_apart = d_k_out == nullptr || d_k_out == d_k || !overlap(d_k_out, kb, d_k, kb);
-    const bool fused = d_q_out == d_q && (d_k_out == nullptr || d_k_out == d_k);
-    const bool others_apart =
-        fused || ((d_q_out == d_q || (!overlap(d_q_out, qb, d_k, kb) && (vb == 0 || !overlap(d_q_out, qb, d_v, vb)))) &&
-                  (d_k_out == nullptr || d_k_out == d_k ||
-                   (!overlap(d_k_out, kb, d_q, qb) && (vb == 0 || !overlap(d_k_out, kb, d_v, vb)))) &&
-                  (d_k_out == nullptr || !overlap(d_q_out, qb, d_k_out, kb)));
-    if (!q_apart || !k_apart || !others_apart) {
+     * v), and an output may be its own input; otherwise no rows share floats. */
+    const int64_t qw = (int64_t)q_heads * head_dim, kw = (int64_t)kv_heads * head_dim;
+    const size_t qb = rows_bytes(tokens, q_stride, qw), kb = rows_bytes(tokens, k_stride, kw);
+    const size_t vb = cache != nullptr ? rows_bytes(tokens, v_stride, kw) : 0;
+    const auto meets_v = [&](const float *out, int64_t stride, int64_t width) {
+        return cache != nullptr && rows_meet(out, stride, width, d_v, v_stride, kw, tokens);
+    };
+    if ((d_q_out != d_q && rows_meet(d_q_out, q_stride, qw, d_q, q_stride, qw, tokens)) ||
+        rows_meet(d_q_out, q_stride, qw, d_k, k_stride, kw, tokens) || meets_v(d_q_out, q_stride, qw) ||
+        (d_k_out != nullptr &&
+         ((d_k_out != d_k && rows_meet(d_k_out, k_stride, kw, d_k, k_stride, kw, tokens)) ||
+          rows_meet(d_k_out, k_stride, kw, d_q, q_stride, qw, tokens) || meets_v(d_k_out, k_stride, kw) ||
+          rows_meet(d_q_out, q_stride, qw, d_k_out, k_stride, kw, tokens)))) {
         set_error("a rotary output overlaps rows other than its own input's");
         return 0;
     }
     if (cache != nullptr) {
         const size_t cb = cache_bytes(*cache);
+        if (cache->keys == cache->values) {
+            set_error("keys and values would be stored in one place");
+            return 0;
+        }
         for (const void *c : {cache->keys, cache->values})
             if (overlap(c, cb, d_q_out, qb) || overlap(c, cb, d_q, qb) || overlap(c, cb, d_k, kb) ||
                 overlap(c, cb, d_v, vb) || (d_k_out != nullptr && overlap(c, cb, d_k_out, kb))) {

@@ -37,6 +37,36 @@ def test_rope_cuts_starts_to_the_tokens(qmv, hip, with_lengths):  # noqa: F811
             assert np.max(np.abs(got[t] - A.rope64(x[t], p, f, False))) <= _rope_bound(x[t]), (t, p)
 
 
+def test_rope_from_one_buffer_into_another(qmv, hip):  # noqa: F811
+    """q, k and v of a token side by side; turned q and k side by side in another
+    buffer; k and v into a cache."""
+    rng = np.random.default_rng(45)
+    heads, kv_heads, dim, b = 6, 2, 64, A.Batch([9, 4], [30, 4], 16, 2)
+    T, wide, out_wide = b.tokens, 10 * 64, 10 * 64
+    rows = _rand(rng, T, wide)
+    f = A.frequencies(dim)
+    blank = [np.full((n, kv_heads, dim), np.nan, np.float32) for n in b.length]
+    cache = A.Cache(qmv, hip, b, blank, blank, A.F32)
+    d, out, df = hip.DeviceBuffer.from_array(rows), hip.DeviceBuffer.from_array(np.zeros((T, out_wide), np.float32)), hip.DeviceBuffer.from_array(f)
+    seq = b.upload(qmv, hip)
+    k, v = 4 * heads * dim, 4 * (heads + kv_heads) * dim
+    qmv.device_rope_append(d.ptr, heads, d.ptr + k, d.ptr + v, kv_heads, dim, T, df.ptr, dim, seq, out.ptr, out.ptr + k, cache.c,
+                           q_stride=wide, k_stride=wide, v_stride=wide)
+    hip.synchronize()
+    assert np.array_equal(d.to_array(np.float32, rows.shape), rows)
+    turned = out.to_array(np.float32, (T, 10, dim))
+    assert (turned[:, 8:] == 0).all()
+    keys, values = cache.read(0), cache.read(1)
+    for s in (0, 1):
+        for i, pos in enumerate(b.positions(s)):
+            t = int(b.starts[s]) + i
+            x = rows[t].reshape(10, dim)
+            assert np.max(np.abs(turned[t, :8] - A.rope64(x[:8], pos, f, False))) <= _rope_bound(x)
+            for h in range(kv_heads):
+                assert np.array_equal(keys[cache.at(s, pos, h)], turned[t, heads + h])
+                assert np.array_equal(values[cache.at(s, pos, h)], x[8 + h])
+
+
 # ---- scores at the ends of the range -----------------------------------------------------
 
 
