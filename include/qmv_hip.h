@@ -410,7 +410,7 @@ typedef struct QmvPagedCache {
  * as it was otherwise (d_status may be null). Tokens at negative positions
  * (more new tokens than the length says) are turned and not stored. Two tokens
  * of a call that are stored in one place leave either.
- * Pointers to floats are aligned to 16 bytes, strides are multiples of 4 under
+ * Pointers to floats are aligned to 16 bytes, to ints to 4, strides are multiples of 4 under
  * 2^31; at most 2^22 tokens, 65535 heads and 2^30 rows of a token and a head.
  */
 int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q_heads,

@@ -79,7 +79,13 @@ bool heads_ok(int tokens, int q_heads, int kv_heads, int head_dim)
     return true;
 }
 
-bool sequences_ok(const QmvSequences *q, bool paged)
+/* Arrays of ints at addresses of ints: scalar loads drop the bits below. */
+bool aligned4(const void *p)
+{
+    return ((uintptr_t)p & 3) == 0;
+}
+
+bool sequences_ok(const QmvSequences *q, bool paged, const int *status)
 {
     if (q == nullptr || q->starts == nullptr || q->count <= 0 || q->count > 65535) {
         set_error("invalid sequences (null, or not 1 to 65535 of them)");
@@ -87,6 +93,10 @@ bool sequences_ok(const QmvSequences *q, bool paged)
     }
     if (paged && (q->lengths == nullptr || q->pages == nullptr || q->table_stride <= 0)) {
         set_error("sequences over a cache need lengths and pages");
+        return false;
+    }
+    if (!aligned4(q->starts) || !aligned4(q->lengths) || (paged && !aligned4(q->pages)) || !aligned4(status)) {
+        set_error("unaligned sequences or status");
         return false;
     }
     return true;
@@ -201,7 +211,7 @@ QMV_API int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q
                                        const QmvPagedCache *cache, int *d_status, void *stream)
 {
     int type = QMV_KV_F32;
-    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, cache != nullptr)) return 0;
+    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, cache != nullptr, d_status)) return 0;
     if (!row_stride_ok(d_q, &q_stride, q_heads, head_dim, "q") ||
         !row_stride_ok(d_k, &k_stride, kv_heads, head_dim, "k") ||
         (cache != nullptr && !row_stride_ok(d_v, &v_stride, kv_heads, head_dim, "v")))
@@ -279,7 +289,7 @@ QMV_API int qmv_device_attention_prompt_f32(const float *d_q, int64_t q_stride, 
                                             int kv_heads, int head_dim, float scale, const QmvSequences *sequences,
                                             float *d_out, int64_t out_stride, void *stream)
 {
-    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, false)) return 0;
+    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, false, nullptr)) return 0;
     if (!row_stride_ok(d_q, &q_stride, q_heads, head_dim, "q") ||
         !row_stride_ok(d_k, &k_stride, kv_heads, head_dim, "k") ||
         !row_stride_ok(d_v, &v_stride, kv_heads, head_dim, "v") ||
@@ -322,7 +332,7 @@ QMV_API int qmv_device_attention_paged_f32(const float *d_q, int64_t q_stride, i
         return 0;
     }
     const int kv_heads = cache->kv_heads, head_dim = cache->head_dim;
-    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, true) ||
+    if (!heads_ok(tokens, q_heads, kv_heads, head_dim) || !sequences_ok(sequences, true, d_status) ||
         !cache_ok(cache, sequences, &type))
         return 0;
     if (!row_stride_ok(d_q, &q_stride, q_heads, head_dim, "q") ||

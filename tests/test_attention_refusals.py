@@ -68,3 +68,18 @@ def test_rope_rows_side_by_side(qmv, no_device):
     for a in ((q, 512, k, 512, v, 512, q, k), (q, 512, k, 512, v, 512, out, out + 4 * 256), (q, 512, k, 512, v, 512, q, 3 * FAR),
               (q, 0, out, 256, out + 4 * 128, 256, q, out)):
         assert "hip" in _rope(qmv, cache, *a), a
+
+
+@pytest.mark.parametrize("change", [{"starts": FAR + 2}, {"lengths": FAR + 1}, {"pages": FAR + 3}, {"status": FAR + 2}], ids=str)
+def test_unaligned_ints(qmv, no_device, change):
+    a = {"starts": FAR, "lengths": FAR, "pages": FAR, "status": FAR, **change}
+    seq = qmv.make_sequences(a["starts"], 2, a["lengths"], a["pages"], 4)
+    cache = qmv.make_paged_cache(8 * FAR, 9 * FAR, qmv.GGML_TYPE_F16, 2, 64, 16, 8)
+    assert qmv.hip_lib().qmv_device_attention_paged_f32(FAR, 0, 3, 4, 0.1, seq, cache, 5 * FAR, 0, a["status"], None) == 0
+    assert "unaligned" in qmv.last_error()
+    assert qmv.hip_lib().qmv_device_rope_append_f32(FAR, 0, 4, 2 * FAR, 0, 3 * FAR, 0, 2, 64, 3, FAR, 64, 0, seq, FAR, 2 * FAR, cache,
+                                                    a["status"], None) == 0
+    assert "unaligned" in qmv.last_error()
+    if "starts" in change:
+        assert qmv.hip_lib().qmv_device_attention_prompt_f32(FAR, 0, 2 * FAR, 0, 3 * FAR, 0, 3, 4, 2, 64, 0.1, seq, 5 * FAR, 0, None) == 0
+        assert "unaligned" in qmv.last_error()
