@@ -10,10 +10,10 @@
  *   one token each of 64 sequences of 1 to 8191 keys, f16 cache: the stream of
  *   keys and values, 494 MB in 98 us with the join, 5.0 TB/s;
  *   a prompt of 8192: the matrix cores, 1.44 T operations (three products of
- *   limbs each) in 1.24 to 1.29 ms, 1.12 PFLOP/s at 2.0 GHz, where the power limit holds
- *   the clock;
+ *   limbs each) in 1.27 to 1.38 ms by box, 1.13 PFLOP/s at best, at 2.0 GHz, where
+ *   the power limit holds the clock;
  *   512 tokens over 16100, f16 cache: the matrix cores, 0.23 T (two products) in
- *   247 us, 0.94 PFLOP/s with the pieces' results and their join;
+ *   245 to 255 us, 0.94 PFLOP/s with the pieces' results and their join;
  *   small calls: their chain of memory round trips (lengths, page table, keys)
  *   and a second launch for the join: one token over 777 keys, 14 and 2 heads of
  *   64, 9 + 3 us.
@@ -760,11 +760,13 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
         return at;
     };
     Raw<TYPE> raw[UNITS][SLOTS];
-    /* Rows that fit one tile read a key once, and leave the caches alone: 64
-     * sequences of 4000 keys, 28 and 4 heads of 128, f16, 108 us without and 97
-     * with, of 1000 keys 35 and 35. Not of fp32, whose lanes take 32 bytes of a line
-     * in two loads (64 of 2000: 129 and 139), nor where row tiles share keys (4
-     * sequences of 8000 under 28 tiles each 38 and 41). */
+    /* Tiles of 16 and 32 rows load past the caches, since most often one tile
+     * reads a key there: 64 sequences of 4000 keys, 28 and 4 heads of 128, f16, 108
+     * us without and 97 with, of 1000 keys 35 and 35. Not of fp32, whose lanes take
+     * 32 bytes of a line in two loads (64 of 2000: 129 and 139), nor tiles of more
+     * rows, which share keys (4 sequences of 8000 under 28 tiles each 38 and 41).
+     * A sequence of several such tiles, in a call whose average chose them, shares
+     * keys all the same, and reads them from memory each time. */
     constexpr bool STREAM = WR == 1 && TYPE != QMV_KV_F32;
     auto unit_block = [&](int u) { return WR == 1 ? u % NB : wr % NB; };
     auto unit_values = [&](int u) { return WR == 1 ? u >= NB : UNITS == 1 ? wr >= NB : u == 1; };
@@ -1176,11 +1178,13 @@ __device__ __forceinline__ void attend_piece(const AttnParams &p, const AttnItem
     }
 }
 
-/* From 32 rows on two waves a SIMD (except where two limbs of 128 elements and
- * their loads do not fit 256 registers beside 32 rows of a wave: 38 would spill;
- * with one, of f16 keys, 32 rows take 149 us for 4 tokens each over 64 sequences
- * of 4000, and 112 with two). At 16 and 32 rows the 4 waves have a tile each in
- * their own LDS and need no barrier. */
+/* From 32 rows on two waves a SIMD, except of fp32 with 128 elements, whose
+ * tiles in LDS leave room for one workgroup (of 4 waves at 32 and 128 rows). Spilled,
+ * of 128 elements: 23 registers of fp32 at 256 rows, 9 of bf16 and 6 of f16 at 32
+ * (with one wave a SIMD none, but 149 us for 4 tokens each over 64 sequences of 4000
+ * f16 keys, 112 with two), and 3 into accumulation registers of fp32 at 16 and 128.
+ * At 16 and 32 rows the 4 waves have a tile each in their own LDS and need no
+ * barrier. */
 template <int TYPE, int DP, int RW, int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK, WR == 8 || (RW == 32 && (TYPE != QMV_KV_F32 || DP == 64)) ? 2 : 1)
 void attention_kernel(AttnParams p)
@@ -1203,8 +1207,7 @@ void attention_kernel(AttnParams p)
     /* A decoding sequence among longer ones: its one tile as the 16-row kernel
      * takes it (512 tokens and 15 decoding sequences of 8000 keys 106 us without, 71
      * with, 2048 and 8 of 6000 182 and 133; 28 and 4 heads of 128, f16). That has its
-     * place in LDS beside the workgroups that run at once, and needs no more
-     * registers (of fp32 under 256 rows 16 spill). */
+     * place in LDS beside the workgroups that run at once. */
     if constexpr (MIXED) {
         if (it.n * (a.heads / a.kv_heads) <= 16) {
             if (threadIdx.x >= 256) return; /* a barrier waits for the waves that are left */
@@ -1326,9 +1329,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnParams p, int s
  *   tokens over 4096 in 8 sequences 124 and 88. Heads of up to 64 are half as
  *   much work per key, and two workgroups of 128 hide more: 8 prompts of 2502
  *   tokens, 14 and 2 heads, 38 and 41.
+ * The average is over all sequences of the call, idle ones too: a chunk beside
+ * many decoding sequences, or in a batch of mostly idle ones, gets the tiles of
+ * those, and a long prompt packed with short ones no images.
  * Pieces (target): as many as run at once, two workgroups a compute unit at
- * 32 and 128 rows and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152 with
- * 512); of 16 rows twice that, because sequences that decode differ in length
+ * 32 and 128 rows (of fp32 keys with more than 64 elements only one does, and the
+ * pieces are two rounds) and one at 256 (prompts of 2048, 7B: 134 with 256 pieces, 152
+ * with 512); of 16 rows twice that, because sequences that decode differ in length
  * most (64 of 1 to 8191 keys: 110 with 1024, 123 with 512), except over fp32,
  * whose tiles leave room for one workgroup. Also twice over a cache where tiles
  * of 128 or 256 alone are more than half of them, unless lengths and new tokens are alike
