@@ -171,10 +171,10 @@ def test_threads_on_per_thread_streams(qmv, hip):  # noqa: F811
 
 def test_a_refused_allocation_leaves_no_error(qmv, hip):  # noqa: F811
     """A call whose workspace the card cannot hold (the images of 2^22 - 64 tokens of
-    256 heads, 1.1 TB) is refused before any launch, so that its addresses are
+    255 heads, 1.1 TB) is refused before any launch, so that its addresses are
     never read; the next call of the thread is not told of it."""
-    tokens, heads = (1 << 22) - 64, 256
-    assert plan(tokens, heads, heads, 128, 1).images * (64 * 128 * 8 + 256) > 1 << 40
+    tokens, heads = (1 << 22) - 64, 255
+    assert plan(tokens, heads, heads, 128, 1).images * (64 * 128 * 8 + 256) > 10 ** 12
     starts = hip.DeviceBuffer.from_array(np.array([0, tokens], np.int32))
     with pytest.raises(qmv.QmvError, match="memory"):
         qmv.device_attention_prompt(1 << 44, 2 << 44, 3 << 44, tokens, heads, heads, 128, 0.1, qmv.make_sequences(starts.ptr, 1), 4 << 44)
