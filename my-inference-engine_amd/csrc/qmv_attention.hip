@@ -10,7 +10,7 @@
  *   one token each of 64 sequences of 1 to 8191 keys, f16 cache: the stream of
  *   keys and values, 494 MB in 98 us with the join, 5.0 TB/s;
  *   a prompt of 8192: the matrix cores, 1.44 T operations (three products of
- *   limbs each) in 1.27 to 1.38 ms by box, 1.13 PFLOP/s at best, at 2.0 GHz, where
+ *   limbs each) in 1.27 to 1.38 ms by card, 1.13 PFLOP/s at best, at 2.0 GHz, where
  *   the power limit holds the clock;
  *   512 tokens over 16100, f16 cache: the matrix cores, 0.23 T (two products) in
  *   245 to 255 us, 0.94 PFLOP/s with the pieces' results and their join;

@@ -295,7 +295,10 @@ Workspace &workspace_for(int device, hipStream_t stream)
         if (slot && slot->thread != t_thread) {
             hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
             const bool captured = hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone;
-            if (captured || hipDeviceSynchronize() != hipSuccess) g_left_workspaces.push_back(std::move(slot));
+            if (captured || hipDeviceSynchronize() != hipSuccess) {
+                (void)hipGetLastError();
+                g_left_workspaces.push_back(std::move(slot));
+            }
         }
     }
     if (!slot) slot.reset(new Workspace());
