@@ -393,9 +393,9 @@ typedef struct QmvPagedCache {
  * Rotary embedding of the new tokens' queries and keys
  * (src/transformer_ops.cpp:43) and the write of keys and values into the cache,
  * what the decode step does after the q/k/v projections. Token t's heads are
- * rows of head_dim floats from d_q + t * q_stride, d_k + t * k_stride and d_v + t
- * * v_stride (a stride of 0: the heads alone); d_q_out and d_k_out have the
- * strides of d_q and d_k and may be them. Other than that an output shares no
+ * rows of head_dim floats, the first at d_q + t * q_stride, d_k + t * k_stride,
+ * d_v + t * v_stride (a stride of 0: the heads alone); d_q_out and d_k_out have
+ * the strides of d_q and d_k and may be them. Other than that an output shares no
  * floats with any of the rows, which may lie side by side in one buffer. Pair i <
  * rotary_dims / 2 of a head at position p turns by the angle p *
  * d_frequencies[i], a product in 64 bits: (x, y) becomes (x cos - y sin, x sin
@@ -410,8 +410,9 @@ typedef struct QmvPagedCache {
  * as it was otherwise (d_status may be null). Tokens at negative positions
  * (more new tokens than the length says) are turned and not stored. Two tokens
  * of a call that are stored in one place leave either.
- * Pointers to floats are aligned to 16 bytes, to ints to 4, strides are multiples of 4 under
- * 2^31; at most 2^22 tokens, 65535 heads and 2^30 rows of a token and a head.
+ * Pointers to floats are aligned to 16 bytes, to ints to 4; strides are multiples
+ * of 4 under 2^31; at most 2^22 tokens, 65535 heads and 2^30 rows of a token and a
+ * head (of attention fewer where they would take 2^32 threads, which is refused).
  */
 int qmv_device_rope_append_f32(const float *d_q, int64_t q_stride, int q_heads,
                                const float *d_k, int64_t k_stride,
